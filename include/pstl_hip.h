@@ -27,14 +27,15 @@
 extern "C" {
 #endif
 
-#define PSTL_ABI_VERSION 6   /* 2: pstl_encode_scene takes a work buffer; --joint and --refinement entry points
+#define PSTL_ABI_VERSION 7   /* 2: pstl_encode_scene takes a work buffer; --joint and --refinement entry points
                                 3: status block in the packed weight buffer (pstl_packed_status_offset)
                                 4: pstl_cfg.dyn -- run-time parameters in device memory (HIP-graph replay)
                                 5: pstl_rollout_layout; chain_waves = 2 (the row-stationary denoiser kernel);
                                    pstl_train_create / pstl_train_destroy and the (empty) context argument of
                                    pstl_refine_backward are gone
                                 6: pstl_cfg.plan_rows (every shard of a job on the same denoiser kernel); pstl_adam_step;
-                                   the prepared lane table's fourth float is the reciprocal segment length */
+                                   the prepared lane table's fourth float is the reciprocal segment length
+                                7: pstl_qk_norm_rope, pstl_attention, pstl_dropout_add and their backward passes */
 
 /* compile-time shape of the path (reference defaults: nt=20, n_segs=15, hiddens=[256,256], feat 7*32) */
 #define PSTL_T 20
@@ -459,6 +460,87 @@ int pstl_refinement(const pstl_cfg* cfg, const float* s0, const float* nei_prep,
                     const float* hl, const float* valid, float thres, float grad_scale, int iters,
                     const float* adam_neg_step, const float* adam_bc2_sqrt, const float* controls, const float* list,
                     int n_list, const int32_t* list_idx, float* work, float* out_controls, float* grad_trace, void* stream);
+
+/* ---- attention over tokens: per-head norm with position rotation, softmax attention, dropout -----------------------
+ * Operators for models of tokens (the scene's ego / neighbour / lane tokens, a trajectory's time steps, long sequences), each
+ * with its backward pass; they stand beside the token encoders above and share the library's Philox generator with
+ * pstl_fill_normal.  Unlike the rest of this header the tensors are of one of three element types, sums are always 32-bit, and
+ * tensors may be strided views.
+ *
+ * A pstl_attn_mat is a (B, L, H, D) tensor whose D elements of a row are consecutive: element (b, l, h, d) is
+ * p[b stride_b + l stride_l + h stride_h + d] (strides in elements, 64-bit).  p and every row start are 16-byte aligned
+ * (PSTL_ERR_ARG otherwise).  Inputs may overlap each other; an output overlaps nothing. */
+enum { PSTL_F32 = 0, PSTL_BF16 = 1, PSTL_F16 = 2 };
+#define PSTL_ATTN_MAX_D 128
+#define PSTL_ROPE_MAX_D 256
+typedef struct pstl_attn_mat {
+  void* p;
+  int64_t stride_b, stride_l, stride_h;
+} pstl_attn_mat;
+
+/* y = rotate(w o x / sqrt(mean_d(x^2) + eps)): q (B,L,Hq,D) and k (B,L,Hk,D) in one launch.  The first `rot` elements of a head
+ * (a multiple of 16, at most D) are rotated in pairs by the angles positions[b pos_stride_b + l] * inv_freq[i], i < rot/2,
+ * formed in 64 bits: pair i is (i, i + rot/2), or (2i, 2i + 1) with `interleaved`; the others are only normalised.
+ * D: a multiple of 8, 8 ... PSTL_ROPE_MAX_D.  Weights, their gradients and work: float32, dense, 16-byte aligned.
+ * Backward (from the ORIGINAL q, k): dq, dk, dwq (D), dwk (D), all written; work: pstl_qk_norm_rope_work_floats floats.
+ * Sums are taken in a fixed order: results repeat bit for bit. */
+typedef struct pstl_qk_rope {
+  int32_t dtype, B, L, Hq, Hk, D, rot, interleaved;
+  float eps;
+  int32_t reserved;
+  pstl_attn_mat q, k, yq, yk;          /* inputs; forward's outputs                  */
+  pstl_attn_mat dyq, dyk, dq, dk;      /* backward: gradients of yq, yk; of q, k     */
+  const float *wq, *wk;                /* (D)                                        */
+  const int64_t* positions;            /* (B,L), or (L) with pos_stride_b = 0        */
+  int64_t pos_stride_b;
+  const double* inv_freq;              /* (rot/2)                                    */
+  float *dwq, *dwk, *work;
+} pstl_qk_rope;
+int pstl_qk_norm_rope(const pstl_qk_rope* a, void* stream);
+size_t pstl_qk_norm_rope_work_floats(const pstl_qk_rope* a);
+int pstl_qk_norm_rope_backward(const pstl_qk_rope* a, void* stream);
+
+/* o = dropout(softmax(scale q k^T over the visible keys)) v.  q, o (B,Lq,Hq,D); k, v (B,Lk,Hk,D); Hk divides Hq and query head
+ * h reads key head h / (Hq/Hk).  D: a multiple of 8, 8 ... PSTL_ATTN_MAX_D.  scale > 0.
+ * Visible: query i < q_lens[b] sees key j < k_lens[b] with key_mask[b mask_stride_b + j] != 0 and, with `causal`,
+ * j <= i + k_lens[b] - q_lens[b] (the sequences' ends are aligned).  Lengths (null: full) are clamped to the tensors; masked or
+ * out-of-length keys, values and query rows may hold anything, NaN included -- but a value that SOME row of the sequence sees
+ * must be finite for the rows that `causal` hides it from.  A row that sees nothing, or i >= q_lens[b], gives o = 0, lse = -inf
+ * and no gradient.
+ * lse (B, Hk, Lq, Hq/Hk) float32, natural logarithm, or null in the forward call; backward reads it.
+ * dropout_256: a probability is dropped with dropout_256 / 256 and the kept ones are scaled by 256 / (256 - dropout_256): byte
+ * j % 4 of word r % 4 of philox4x32-7(counter = (j / 4, r / 4, b Hk + hk, 0x41545444), key = seed) below dropout_256 drops key j
+ * for packed row r = i Hq/Hk + (h % (Hq/Hk)).  seed_dev (null, or 8 bytes of device memory such as a pstl_dyn) replaces seed at
+ * run time.  The mask is never stored: backward draws it again from the same seed.
+ * work: pstl_attention_work_floats floats (0: null allowed) / pstl_attention_backward_work_floats, 16-byte aligned, used until
+ * the call's kernels have run; two calls in flight at once need one each.
+ * Backward reads q, k, v, o, lse, dout and writes dq, dk, dv whole (zeros behind the lengths and for hidden keys); no atomics:
+ * results repeat bit for bit.  For PSTL_F16 the gradient of a score is held in half precision as an operand. */
+typedef struct pstl_attn {
+  int32_t dtype, B, Lq, Lk, Hq, Hk, D, causal;
+  float scale;
+  int32_t dropout_256;
+  uint64_t seed;
+  const uint64_t* seed_dev;
+  pstl_attn_mat q, k, v, o;
+  pstl_attn_mat dout, dq, dk, dv;
+  float* lse;
+  const uint8_t* key_mask;
+  int64_t mask_stride_b;
+  const int32_t *q_lens, *k_lens;      /* (B) */
+  float* work;
+} pstl_attn;
+size_t pstl_attention_work_floats(const pstl_attn* a);
+int pstl_attention(const pstl_attn* a, void* stream);
+size_t pstl_attention_backward_work_floats(const pstl_attn* a);
+int pstl_attention_backward(const pstl_attn* a, void* stream);
+
+/* y = residual + m x 65536 / (65536 - threshold), n consecutive elements, residual may be null (the backward pass: x = dy);
+ * element e is dropped when its 16 bits -- bits 16 (t % 2) .. of word (t % 8) / 2 of philox4x32-7(counter = (t / 8 low, high,
+ * 0, 0x44524F50), key = seed), t = e + offset -- are below `threshold` (65536: everything is dropped).  `offset` lets parts of
+ * a tensor, or several tensors, share one seed.  seed_dev as above.  y may be x or residual. */
+int pstl_dropout_add(int dtype, int64_t n, const void* x, const void* residual, void* y, int threshold, int64_t seed,
+                     const uint64_t* seed_dev, int64_t offset, void* stream);
 
 #ifdef __cplusplus
 }

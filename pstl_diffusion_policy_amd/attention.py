@@ -1,0 +1,443 @@
+"""Attention over tokens on MI355X: per-head norm with position rotation, softmax attention, dropout -- each with its gradient.
+
+Operators for models of tokens (a scene's ego / neighbour / lane tokens, the time steps of a trajectory, long sequences), beside
+the token encoders of engine.Sampler / engine.RectTrainer.  All arithmetic runs in libpstl_hip.so (csrc/attention_kernels.hip,
+attention_bwd_kernels.hip, token_kernels.hip); tensors are float32, bfloat16 or float16, sums are 32-bit whatever the type.
+
+  qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq)      rotate(w o x / rms(x)) for queries and keys, one launch
+  attention(q, k, v, ...)                                          softmax(scale q k^T) v over padded, ragged, grouped-head batches
+  dropout_add(x, p, seed=...)                                      residual + dropout(x); the mask is a function of (seed, element)
+
+The three work under torch.autograd.  `attention_forward` / `attention_backward`, `qk_norm_rope_forward` /
+`qk_norm_rope_backward` and `dropout_backward` are the same calls without autograd, for hosts that sequence launches themselves
+(a training step captured in a HIP graph: engine.GraphCapture).  Every call only enqueues launches on the current stream of the
+tensors' device -- no synchronisation, no host copy -- and can be captured; call it once before capturing.
+
+A seed is an int, or a tensor in device memory that the kernels read when they RUN (int64, one element, or the block of an
+engine.DynBlock): a captured step draws another mask at each replay.  It must keep its value until the backward pass has run.
+
+There is no CPU path: tensors must live on the GPU and the library must be built (ffi.lib() raises otherwise).
+"""
+import ctypes
+import math
+
+import torch
+
+from . import ffi
+
+_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_HEAD_DIM = 128            # attention (include/pstl_hip.h, PSTL_ATTN_MAX_D)
+MAX_ROPE_HEAD_DIM = 256       # qk_norm_rope (PSTL_ROPE_MAX_D)
+_NO_MAT = (None, 0, 0, 0)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# arguments
+# ---------------------------------------------------------------------------------------------------------------
+def _rows(name, t, like=None):
+    """Checks a (B, L, H, D) operand."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a tensor, got %s" % (name, type(t).__name__))
+    if t.dtype not in _CODES:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    if t.dim() != 4:
+        raise ValueError("%s must be (B, L, H, D), got %s" % (name, tuple(t.shape)))
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError("%s is %s, the queries are %s" % (name, t.dtype, like.dtype))
+        if t.device != like.device:
+            raise ValueError("%s is on %s, the queries are on %s" % (name, t.device, like.device))
+
+
+def _aligned(t):
+    """Can the kernels read t's rows 16 bytes at a time?"""
+    el = t.element_size()
+    sb, sl, sh, sd = t.stride()
+    return sd == 1 and t.data_ptr() % 16 == 0 and (sb * el) % 16 == 0 and (sl * el) % 16 == 0 and (sh * el) % 16 == 0
+
+
+def _on_gpu(*tensors):
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("attention operators run in libpstl_hip.so on the GPU; got a %s tensor" % t.device)
+
+
+def _check_aligned(name, t):
+    if t.numel() and not _aligned(t):
+        raise ValueError("%s: the elements of a row must be consecutive and every row 16-byte aligned (shape %s, strides %s, "
+                         "address mod 16 = %d); pass %s.contiguous()" % (name, tuple(t.shape), t.stride(), t.data_ptr() % 16, name))
+
+
+def _mat(t):
+    if t is None:
+        return _NO_MAT
+    sb, sl, sh, _ = t.stride()
+    return (t.data_ptr(), sb, sl, sh)
+
+
+def _gradient(t, like):
+    """An incoming gradient in a layout the kernels read (autograd hands over expanded and transposed ones)."""
+    if t.dtype != like.dtype:
+        t = t.to(like.dtype)
+    return t if not t.numel() or _aligned(t) else t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _seed(seed, device):
+    """(value, device tensor or None)"""
+    if isinstance(seed, torch.Tensor):
+        dyn = seed.dtype == torch.float32 and seed.numel() == 4
+        if not dyn and not (seed.dtype == torch.int64 and seed.numel() == 1):
+            raise TypeError("a seed tensor holds one int64 (or is the four float32 words of an engine.DynBlock), got %s %s"
+                            % (seed.dtype, tuple(seed.shape)))
+        if seed.device != device or not seed.is_contiguous() or seed.data_ptr() % 8:
+            raise ValueError("a seed tensor lives on the operands' device (%s), contiguous and 8-byte aligned" % device)
+        return 0, seed
+    if isinstance(seed, bool) or not isinstance(seed, int):
+        raise TypeError("seed must be an int or a device tensor, got %s" % type(seed).__name__)
+    return seed & (2 ** 64 - 1), None
+
+
+class _on_device:
+    """The operands' device as the current one, if it is not already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# per-head norm + rotation
+# ---------------------------------------------------------------------------------------------------------------
+def rope_frequencies(rot_dim, base=10000.0, device=None):
+    """The usual table base^(-2 i / rot_dim), i < rot_dim / 2, in float64 (the angles are formed in 64 bits)."""
+    if rot_dim < 16 or rot_dim % 16:
+        raise ValueError("rot_dim must be a positive multiple of 16, got %d" % rot_dim)
+    return float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+
+
+def _rope_checks(q, k, q_weight, k_weight, positions, inv_freq):
+    _rows("q", q)
+    _rows("k", k, q)
+    B, L, Hq, D = q.shape
+    if k.shape[0] != B or k.shape[1] != L or k.shape[3] != D:
+        raise ValueError("q and k must share B, L and D: %s against %s" % (tuple(q.shape), tuple(k.shape)))
+    if Hq < 1 or k.shape[2] < 1:
+        raise ValueError("q and k need at least one head")
+    if D % 8 or not 8 <= D <= MAX_ROPE_HEAD_DIM:
+        raise ValueError("the head dimension must be a multiple of 8 up to %d, got %d" % (MAX_ROPE_HEAD_DIM, D))
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype != torch.float32:
+            raise TypeError("%s must be float32 (the framework's parameters are), got %s" % (name, w.dtype))
+        if tuple(w.shape) != (D,) or w.stride(0) != 1 or w.device != q.device:
+            raise ValueError("%s must be (%d,), contiguous, on %s" % (name, D, q.device))
+    if positions.dtype != torch.int64:
+        raise TypeError("positions must be int64, got %s" % positions.dtype)
+    if tuple(positions.shape) not in ((L,), (B, L)) or positions.device != q.device or (L > 1 and positions.stride(-1) != 1):
+        raise ValueError("positions must be (L,) or (B, L) = (%d, %d) with consecutive elements, on %s" % (B, L, q.device))
+    if inv_freq.dtype != torch.float64:
+        raise TypeError("inv_freq must be float64, got %s" % inv_freq.dtype)
+    rot = 2 * inv_freq.numel()
+    if inv_freq.dim() != 1 or rot < 16 or rot % 16 or rot > D or not inv_freq.is_contiguous() or inv_freq.device != q.device:
+        raise ValueError("inv_freq must be (rot/2,), rot a multiple of 16 up to D = %d, contiguous, on %s" % (D, q.device))
+    _on_gpu(q, q_weight, positions, inv_freq)
+    for name, t in (("q", q), ("k", k)):
+        _check_aligned(name, t)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.data_ptr() % 16:
+            raise ValueError("%s must be 16-byte aligned" % name)
+
+
+def _rope_struct(q, k, wq, wk, positions, inv_freq, eps, interleaved, yq=None, yk=None, dyq=None, dyk=None, dq=None, dk=None,
+                 dwq=None, dwk=None, work=None):
+    B, L, Hq, D = q.shape
+    p = lambda t: None if t is None else t.data_ptr()
+    return ffi.QkRope(_CODES[q.dtype], B, L, Hq, k.shape[2], D, 2 * inv_freq.numel(), int(bool(interleaved)), eps, 0, _mat(q),
+                      _mat(k), _mat(yq), _mat(yk), _mat(dyq), _mat(dyk), _mat(dq), _mat(dk), wq.data_ptr(), wk.data_ptr(),
+                      positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0, inv_freq.data_ptr(), p(dwq),
+                      p(dwk), p(work))
+
+
+def qk_norm_rope_forward(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """qk_norm_rope without autograd."""
+    _rope_checks(q, k, q_weight, k_weight, positions, inv_freq)
+    with _on_device(q.device):
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        a = _rope_struct(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, yq, yk)
+        ffi.check(ffi.lib().pstl_qk_norm_rope(ctypes.byref(a), ffi.stream()), "qk_norm_rope")
+    return yq, yk
+
+
+def qk_norm_rope_backward(dyq, dyk, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rope, from its ORIGINAL inputs and the gradients of its outputs."""
+    _rope_checks(q, k, q_weight, k_weight, positions, inv_freq)
+    for name, t, x in (("dyq", dyq, q), ("dyk", dyk, k)):
+        if t.shape != x.shape or t.device != x.device:
+            raise ValueError("%s must be %s on %s" % (name, tuple(x.shape), x.device))
+    with _on_device(q.device):
+        dyq, dyk = _gradient(dyq, q), _gradient(dyk, k)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+        a = _rope_struct(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, None, None, dyq, dyk, dq, dk, dwq, dwk)
+        work = torch.empty(ffi.lib().pstl_qk_norm_rope_work_floats(ctypes.byref(a)), dtype=torch.float32, device=q.device)
+        a.work = work.data_ptr()
+        ffi.check(ffi.lib().pstl_qk_norm_rope_backward(ctypes.byref(a), ffi.stream()), "qk_norm_rope_backward")
+    return dq, dk, dwq, dwk
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, positions, inv_freq, eps, interleaved):
+        ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
+        ctx.opts = (eps, interleaved)
+        return qk_norm_rope_forward(q, k, wq, wk, positions, inv_freq, eps, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dyq, dyk):
+        return qk_norm_rope_backward(dyq, dyk, *ctx.saved_tensors, *ctx.opts) + (None,) * 4
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """Queries and keys, each normalised per head and rotated by position: rotate(w o x / sqrt(mean(x^2) + eps)) -> (yq, yk).
+
+    q (B, L, Hq, D), k (B, L, Hk, D), D a multiple of 8 up to 256; views of a fused projection are read in place.  q_weight,
+    k_weight (D,) float32.  positions (L,) or (B, L) int64.  inv_freq (rot/2,) float64 (rope_frequencies): the first rot elements
+    of a head are rotated, pair i = (i, i + rot/2) or, interleaved, (2i, 2i + 1), by positions * inv_freq[i]; the others are only
+    normalised.  Differentiable in q, k and the weights."""
+    if _needs_grad(q, k, q_weight, k_weight):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    return qk_norm_rope_forward(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------
+def _attn_checks(q, k, v, key_mask, q_lens, k_lens, dropout_p):
+    """Checks the operands; returns the dropout probability in 256ths."""
+    _rows("q", q)
+    _rows("k", k, q)
+    _rows("v", v, q)
+    B, Lq, Hq, D = q.shape
+    Lk, Hk = k.shape[1], k.shape[2]
+    if tuple(k.shape) != (B, Lk, Hk, D) or v.shape != k.shape:
+        raise ValueError("k and v must be (B, Lk, Hk, D) with the queries' B and D: q %s, k %s, v %s"
+                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError("the key heads (%d) must divide the query heads (%d)" % (Hk, Hq))
+    if D % 8 or not 8 <= D <= MAX_HEAD_DIM:
+        raise ValueError("the head dimension must be a multiple of 8 up to %d, got %d" % (MAX_HEAD_DIM, D))
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8):
+            raise TypeError("key_mask must be bool or uint8 (true = visible), got %s" % key_mask.dtype)
+        if tuple(key_mask.shape) != (B, Lk) or key_mask.device != q.device or (Lk > 1 and key_mask.stride(1) != 1):
+            raise ValueError("key_mask must be (B, Lk) = (%d, %d) with consecutive elements, on %s" % (B, Lk, q.device))
+    for name, t in (("q_lens", q_lens), ("k_lens", k_lens)):
+        if t is None:
+            continue
+        if t.dtype != torch.int32:
+            raise TypeError("%s must be int32, got %s" % (name, t.dtype))
+        if tuple(t.shape) != (B,) or t.device != q.device or not t.is_contiguous():
+            raise ValueError("%s must be (B,) = (%d,), contiguous, on %s" % (name, B, q.device))
+    if not 0.0 <= dropout_p < 1.0:
+        raise ValueError("dropout_p must be in [0, 1), got %r" % (dropout_p,))
+    n256 = int(round(256 * dropout_p))
+    if dropout_p > 0.0 and not 1 <= n256 <= 255:
+        raise ValueError("dropout_p is realised in steps of 1/256, from 1/256 to 255/256; got %r" % (dropout_p,))
+    _on_gpu(q)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check_aligned(name, t)
+    return n256
+
+
+def _attn_scale(scale, D):
+    if scale is None:
+        return 1.0 / math.sqrt(D)
+    scale = float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite, got %r" % (scale,))
+    return scale
+
+
+def _attn_struct(q, k, v, o, causal, scale, n256, seed, seed_dev, key_mask, q_lens, k_lens, lse=None, dout=None, dq=None,
+                 dk=None, dv=None):
+    B, Lq, Hq, D = q.shape
+    p = lambda t: None if t is None else t.data_ptr()
+    return ffi.Attn(_CODES[q.dtype], B, Lq, k.shape[1], Hq, k.shape[2], D, int(bool(causal)), scale, n256, seed, p(seed_dev),
+                    _mat(q), _mat(k), _mat(v), _mat(o), _mat(dout), _mat(dq), _mat(dk), _mat(dv), p(lse), p(key_mask),
+                    0 if key_mask is None else key_mask.stride(0), p(q_lens), p(k_lens), None)
+
+
+def attention_forward(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, scale=None, dropout_p=0.0, seed=0,
+                      need_lse=True):
+    """attention without autograd: (out, lse).  lse (B, Hk, Lq, Hq/Hk) float32 is what attention_backward takes (None with
+    need_lse=False)."""
+    n256 = _attn_checks(q, k, v, key_mask, q_lens, k_lens, dropout_p)
+    scale = _attn_scale(scale, q.shape[3])
+    seed, seed_dev = _seed(seed, q.device)
+    B, Lq, Hq, _ = q.shape
+    Hk = k.shape[2]
+    with _on_device(q.device):
+        L = ffi.lib()
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((B, Hk, Lq, Hq // Hk), dtype=torch.float32, device=q.device) if need_lse else None
+        a = _attn_struct(q, k, v, out, causal, scale, n256, seed, seed_dev, key_mask, q_lens, k_lens, lse)
+        ref = ctypes.byref(a)
+        n = L.pstl_attention_work_floats(ref)
+        if n:
+            work = torch.empty(n, dtype=torch.float32, device=q.device)
+            a.work = work.data_ptr()
+        ffi.check(L.pstl_attention(ref, ffi.stream()), "attention")
+    return out, lse
+
+
+def attention_backward(dout, q, k, v, out, lse, causal=False, key_mask=None, q_lens=None, k_lens=None, scale=None,
+                       dropout_p=0.0, seed=0):
+    """(dq, dk, dv) of attention, from its inputs, its results and the gradient of `out`.  Deterministic: no atomics."""
+    n256 = _attn_checks(q, k, v, key_mask, q_lens, k_lens, dropout_p)
+    scale = _attn_scale(scale, q.shape[3])
+    seed, seed_dev = _seed(seed, q.device)
+    B, Lq, Hq, _ = q.shape
+    Hk = k.shape[2]
+    for name, t in (("dout", dout), ("out", out)):
+        if t.shape != q.shape or t.device != q.device:
+            raise ValueError("%s must be %s on %s" % (name, tuple(q.shape), q.device))
+    if (out.dtype != q.dtype or lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hk, Lq, Hq // Hk) or not lse.is_contiguous()
+            or lse.device != q.device):
+        raise ValueError("out (%s) and lse (float32, %s) are what attention_forward returned" % (q.dtype, (B, Hk, Lq, Hq // Hk)))
+    _check_aligned("out", out)
+    with _on_device(q.device):
+        L = ffi.lib()
+        dout = _gradient(dout, q)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        a = _attn_struct(q, k, v, out, causal, scale, n256, seed, seed_dev, key_mask, q_lens, k_lens, lse, dout, dq, dk, dv)
+        ref = ctypes.byref(a)
+        work = torch.empty(L.pstl_attention_backward_work_floats(ref), dtype=torch.float32, device=q.device)
+        a.work = work.data_ptr()
+        ffi.check(L.pstl_attention_backward(ref, ffi.stream()), "attention_backward")
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed):
+        out, lse = attention_forward(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed)
+        on_device = isinstance(seed, torch.Tensor)
+        # (saved, so that autograd refuses a backward pass whose masks, lengths or seed were overwritten in between)
+        ctx.save_for_backward(q, k, v, out, lse, key_mask, q_lens, k_lens, seed if on_device else None)
+        ctx.opts = (causal, scale, dropout_p, None if on_device else seed)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 10
+        q, k, v, out, lse, key_mask, q_lens, k_lens, seed_dev = ctx.saved_tensors
+        causal, scale, dropout_p, seed = ctx.opts
+        return attention_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, scale, dropout_p,
+                                  seed if seed_dev is None else seed_dev) + (None,) * 7
+
+
+def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, scale=None, dropout_p=0.0, seed=0,
+              return_lse=False):
+    """softmax(scale q k^T over the visible keys) v -> (B, Lq, Hq, D).
+
+    q (B, Lq, Hq, D), k and v (B, Lk, Hk, D): Hk divides Hq (query head h reads key head h // (Hq/Hk)), D a multiple of 8 up to
+    128.  Strided views are read in place (rows 16-byte aligned): a cache of Lk slots, a fused projection, (B, H, L, D) tensors
+    transposed.  scale: 1/sqrt(D) by default.
+    A query sees the keys j < k_lens[b] ((B,) int32; Lk) that key_mask ((B, Lk) bool / uint8, true = visible) shows it and, with
+    causal, j <= i + k_lens[b] - q_lens[b]: the ends of the sequences are aligned, so a single new query sees its whole cache.
+    Queries i >= q_lens[b] and queries that see nothing give zeros, and no gradient.  What is hidden by the mask or lies behind the
+    lengths may hold anything.
+    dropout_p drops probabilities (steps of 1/256; kept ones are scaled by the inverse of the realised keep probability), seed
+    draws the mask.  return_lse: also the log of the softmax's sums, (B, Hq, Lq) float32, without a gradient.
+    Differentiable in q, k and v; the backward pass forms the probabilities again and is deterministic."""
+    if _needs_grad(q, k, v):
+        out, lse = _Attention.apply(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed)
+    else:
+        out, lse = attention_forward(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed, need_lse=return_lse)
+    if not return_lse:
+        return out
+    B, Lq, Hq, _ = q.shape
+    return out, lse.permute(0, 1, 3, 2).reshape(B, Hq, Lq)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# dropout
+# ---------------------------------------------------------------------------------------------------------------
+def _dropout_launch(x, residual, p, seed, offset):
+    value, seed_dev = _seed(seed, x.device)
+    _on_gpu(x)
+    with _on_device(x.device):
+        x = x.contiguous()
+        residual = None if residual is None else residual.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        q = lambda t: None if t is None else t.data_ptr()
+        ffi.check(ffi.lib().pstl_dropout_add(_CODES[x.dtype], x.numel(), x.data_ptr(), q(residual), y.data_ptr(),
+                                             int(round(65536 * p)), value - 2 ** 64 if value >= 2 ** 63 else value, q(seed_dev),
+                                             offset, ffi.stream()), "dropout_add")
+    return y
+
+
+def _dropout_checks(x, p, offset, residual):
+    if x.dtype not in _CODES:
+        raise TypeError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("p must be in [0, 1], got %r" % (p,))
+    if isinstance(offset, bool) or not isinstance(offset, int) or not 0 <= offset < 2 ** 62:
+        raise ValueError("offset must be an int in [0, 2^62), got %r" % (offset,))
+    if residual is not None:
+        if residual.dtype != x.dtype:
+            raise TypeError("residual is %s, x is %s" % (residual.dtype, x.dtype))
+        if residual.shape != x.shape or residual.device != x.device:
+            raise ValueError("residual must be %s on %s" % (tuple(x.shape), x.device))
+
+
+def dropout_backward(dy, p, seed, offset=0):
+    """The gradient of dropout_add in x: the same mask on dy (its gradient in the residual is dy itself)."""
+    _dropout_checks(dy, p, offset, None)
+    return _dropout_launch(dy, None, p, seed, offset)
+
+
+class _DropoutAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        on_device = isinstance(seed, torch.Tensor)
+        ctx.save_for_backward(seed if on_device else None)
+        ctx.opts = (p, None if on_device else seed, offset)
+        return _dropout_launch(x, residual, p, seed, offset)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        p, seed, offset = ctx.opts
+        seed_dev, = ctx.saved_tensors
+        dx = _dropout_launch(dy, None, p, seed if seed_dev is None else seed_dev, offset) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout_add(x, p, seed, offset=0, residual=None):
+    """residual + dropout(x): every element of x is dropped with probability p (to 1/65536), the kept ones are scaled by the
+    inverse of the realised keep probability.  The mask is a function of (seed, offset + index of the element in x's order) and is
+    drawn again by the backward pass.  offset lets several tensors (or the shards of one) share a seed.  residual: x's shape
+    and type, or None.  Differentiable in x and residual."""
+    _dropout_checks(x, p, offset, residual)
+    if _needs_grad(x, residual):
+        return _DropoutAdd.apply(x, residual, p, seed, offset)
+    return _dropout_launch(x, residual, p, seed, offset)

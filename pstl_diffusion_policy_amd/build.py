@@ -14,6 +14,7 @@ ARCH = "gfx950"
 # scheduled with the ILP-oriented machine scheduler: the default one serialises chains of packed-fp32 operations through
 # one temporary and pays an s_nop between every two of them (a third of the issue slots of the circle-pair loop);
 # results are bit-identical, the guidance kernel is 3 % faster.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 UNITS = [("stl_kernels.hip", ["-ffp-contract=off", "-Xarch_device", "-mllvm=-misched=gcn-iterative-ilp"]),
          # mlp_kernels: top-down pre-RA list scheduling follows the hand-laid order of the chain kernel's fused block more
          # closely (multi-step launch -1.4 %, single-step -1.9 %, nothing else in the unit changes)
@@ -26,7 +27,10 @@ UNITS = [("stl_kernels.hip", ["-ffp-contract=off", "-Xarch_device", "-mllvm=-mis
          ("chain2_kernels.hip", ["-Xarch_device", "-mllvm=-amdgpu-mfma-vgpr-form", "-DPSTL_C2_PART=2"], "chain2_kernels_p2.o"),
          ("diversity_kernels.hip", ["-ffp-contract=off"]), ("stl_program.hip", ["-ffp-contract=off"]),
          # adam_kernels: torch.optim.Adam's float32 update, every operation rounded on its own (csrc/adam_core.hpp)
-         ("adam_kernels.hip", ["-ffp-contract=off"])]
+         ("adam_kernels.hip", ["-ffp-contract=off"]),
+         # attention over tokens (no packed fp32 instructions)
+         ("attention_kernels.hip", NO_PACKED_FP32), ("attention_bwd_kernels.hip", NO_PACKED_FP32),
+         ("token_kernels.hip", NO_PACKED_FP32)]
 LINK_LIBS = []   # no vendor BLAS: every kernel of the library is in csrc/
 
 

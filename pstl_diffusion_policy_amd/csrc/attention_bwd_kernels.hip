@@ -1,0 +1,419 @@
+// attention_bwd_kernels.hip -- softmax attention, backward: the probabilities are formed again from q, k and the saved lse.
+//
+//   P = exp(S - lse);  delta_r = sum_d dO_rd O_rd;  dV = (m P / keep)^T dO;  dP = dO V^T;  dS = P o (m dP / keep - delta)
+//   dQ = scale dS K;   dK = scale dS^T Q
+// Two launches without atomics, so that a result does not depend on the order in which workgroups finish: k_attn_bwd_q (a lane
+// holds one row: S^T, dP^T, dQ^T; it also leaves delta) and k_attn_bwd_kv (a lane holds one key: S, dP, dK^T, dV^T; packed rows
+// make the sum over the heads that share a key head part of the same accumulator).  S and dP are formed in both: seven products
+// instead of five, against a second pass over dQ in memory.  Sequences of at most 32 keys have one launch (k_attn_bwd_short).
+// Arithmetic: P and dS are rounded to the inputs' type as operands of dV, dQ and dK; all sums are 32-bit.
+#include "attn_host.hpp"
+
+namespace pstl {
+namespace attn {
+namespace {
+
+template <typename T>
+constexpr int block_len() {
+  return sizeof(T) == 2 ? 64 : 32;
+}
+template <typename T, int DK>
+constexpr int waves_per_simd() {
+  return (sizeof(T) == 2 && DK <= 64) || DK <= 32 ? 2 : 1;
+}
+
+// sum over d of the product of two rows (row fragments; both lane halves)
+template <typename T, int DK>
+__device__ inline float row_dot(const Frag<T> (&x)[DK / 16], const Frag<T> (&y)[DK / 16]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = __builtin_fmaf((float)x[t][j], (float)y[t][j], s);
+  return half_sum(s);
+}
+
+// ---- dQ: 128 packed rows per workgroup -------------------------------------------------------------------------------
+template <typename T, int DK, bool DROP>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_q(Args a) {
+  constexpr int W = lds_width(DK), BN = block_len<T>(), NS = BN / 32;
+  typedef Tile<T, W> TL;
+  constexpr int kTileBytes = BN * TL::kRowBytes, kPer = BN * TL::kChunks / 256;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, col = lane & 31;
+  const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const int unit = work / a.n_tiles, tile = a.n_tiles - 1 - (work - unit * a.n_tiles);
+  const int b = unit / a.Hk, hk = unit - b * a.Hk;
+  const Lens n = lens_of(a, b);
+  const int r0 = tile * 128 + wave * 32, r = r0 + col;
+  const int qi = row_query(a, r);
+  const bool live = r < a.R && qi < n.q;
+  const int lim = live ? row_limit(a, n, qi) : 0;
+  const int q_first = row_query(a, tile * 128), q_last = min(row_query(a, min(tile * 128 + 127, a.R - 1)), n.q - 1);
+  const int kend = q_first < n.q ? row_limit(a, n, q_last) : 0;
+  const int q_wave = row_query(a, r0);
+  const int all_see = r0 + 32 > a.R || row_query(a, r0 + 31) >= n.q ? 0 : a.causal ? max(min(q_wave + n.k - n.q + 1, n.k), 0) : n.k;
+
+  Frag<T> qf[DK / 16], dof[DK / 16];
+  load_row_frags<T, DK>(live ? row_ptr<T>(a, a.q, b, hk, r) : nullptr, live, a.D, hi, qf);
+  load_row_frags<T, DK>(live ? row_ptr<T>(a, a.dout, b, hk, r) : nullptr, live, a.D, hi, dof);
+  float delta, lse2;
+  {
+    Frag<T> of[DK / 16];
+    load_row_frags<T, DK>(live ? row_ptr<T>(a, a.o, b, hk, r) : nullptr, live, a.D, hi, of);
+    delta = row_dot<T, DK>(dof, of);
+    lse2 = live ? a.lse[(int64_t)unit * a.R + r] * kLog2e : 0.0f;
+    if (hi == 0 && r < a.R) a.delta[(int64_t)unit * a.R + r] = delta;
+  }
+  f32x16 acc[DK / 32] = {};
+  const uint64_t seed = DROP ? drop_seed(a) : 0;
+
+  u32x4v stage[2][kPer];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = tid + 256 * i, row = id / TL::kChunks, c = (id % TL::kChunks) ^ TL::swz(row), key = k0 + row;
+      const int d = c * TL::kChunkEl;
+      bool ok = key < n.k && d < a.D;
+      if (ok && a.key_mask) ok = a.key_mask[b * a.mask_sb + key] != 0;
+      stage[0][i] = ok ? *reinterpret_cast<const u32x4v*>(key_ptr<T>(a.k, b, hk, key) + d) : u32x4v{0, 0, 0, 0};
+      stage[1][i] = ok ? *reinterpret_cast<const u32x4v*>(key_ptr<T>(a.v, b, hk, key) + d) : u32x4v{0, 0, 0, 0};
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      *reinterpret_cast<u32x4v*>(&lds[buf][0][(tid + 256 * i) * 16]) = stage[0][i];
+      *reinterpret_cast<u32x4v*>(&lds[buf][1][(tid + 256 * i) * 16]) = stage[1][i];
+    }
+  };
+  if (kend > 0) {
+    fetch(0);
+    store(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
+    const bool more = k0 + BN < kend;
+    if (more) fetch(k0 + BN);
+    const char *kt = lds[buf][0], *vt = lds[buf][1];
+    const bool masked = k0 + BN > all_see || a.key_mask;
+    uint64_t vis = ~0ull;
+    if (a.key_mask) {
+      const int key = k0 + lane;
+      vis = __ballot(key < n.k && lane < BN && a.key_mask[b * a.mask_sb + key] != 0) >> (4 * hi);
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(kt, 32 * j + col, t, hi), qf[t], s);
+#pragma unroll
+      for (int t = 0; t < DK / 16; ++t) dp = mma(TL::row(vt, 32 * j + col, t, hi), dof[t], dp);
+      uint32_t w[4];
+      if (DROP) drop_words_rows(seed, (uint32_t)unit, r, k0 + 32 * j, lane, w);
+#pragma unroll
+      for (int g = 0; g < 16; ++g) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse2));
+        float dpv = dp[g];
+        if (DROP) dpv = kept(w, g, a.thr) ? dpv * a.keep_inv : 0.0f;
+        s[g] = p * (dpv - delta);
+      }
+      if (masked) {
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+          const int o = 32 * j + 8 * (g >> 2) + (g & 3);
+          const bool see = k0 + o + 4 * hi < lim && ((vis >> o) & 1);
+          s[g] = see ? s[g] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const Frag<T> ds = acc_frag<T>(s, t);
+#pragma unroll
+        for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = mma(TL::col(kt, 32 * j + 16 * t, dt, lane), ds, acc[dt]);
+      }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+  if (r >= a.R) return;
+  store_col<T, DK>(row_ptr<T>(a, a.dq, b, hk, r), a.D, hi, acc, live ? a.scale : 0.0f);
+}
+
+// ---- dK, dV: 128 keys per workgroup ------------------------------------------------------------------------------------
+template <typename T, int DK, bool DROP>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_kv(Args a) {
+  constexpr int W = lds_width(DK), BM = block_len<T>(), NS = BM / 32;
+  typedef Tile<T, W> TL;
+  constexpr int kTileBytes = BM * TL::kRowBytes, kPer = BM * TL::kChunks / 256;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
+  __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM];
+  __shared__ __attribute__((aligned(16))) int row_lim[2][BM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, col = lane & 31;
+  const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const int unit = work / a.n_tiles, tile = work - unit * a.n_tiles;      // (causal: the first keys are seen by the most rows)
+  const int b = unit / a.Hk, hk = unit - b * a.Hk;
+  const Lens n = lens_of(a, b);
+  const int key = tile * 128 + wave * 32 + col;
+  const bool live = key < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + key] != 0);
+  const int r_end = tile * 128 < n.k ? n.q * a.G : 0;
+  const int r_begin = a.causal ? max(tile * 128 - (n.k - n.q), 0) * a.G / BM * BM : 0;
+
+  Frag<T> kf[DK / 16], vf[DK / 16];
+  load_row_frags<T, DK>(live ? key_ptr<T>(a.k, b, hk, key) : nullptr, live, a.D, hi, kf);
+  load_row_frags<T, DK>(live ? key_ptr<T>(a.v, b, hk, key) : nullptr, live, a.D, hi, vf);
+  f32x16 dk[DK / 32] = {}, dv[DK / 32] = {};
+  const uint64_t seed = DROP ? drop_seed(a) : 0;
+
+  u32x4v stage[2][kPer];
+  float st_lse, st_delta;
+  int st_lim;
+  auto fetch = [&](int m0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = tid + 256 * i, row = id / TL::kChunks, d = ((id % TL::kChunks) ^ TL::swz(row)) * TL::kChunkEl, r = m0 + row;
+      const bool ok = r < r_end && d < a.D;
+      stage[0][i] = ok ? *reinterpret_cast<const u32x4v*>(row_ptr<T>(a, a.q, b, hk, r) + d) : u32x4v{0, 0, 0, 0};
+      stage[1][i] = ok ? *reinterpret_cast<const u32x4v*>(row_ptr<T>(a, a.dout, b, hk, r) + d) : u32x4v{0, 0, 0, 0};
+    }
+    if (tid < BM) {
+      const int r = m0 + tid;
+      const bool ok = r < r_end;
+      st_lse = ok ? a.lse[(int64_t)unit * a.R + r] * kLog2e : 0.0f;
+      st_delta = ok ? a.delta[(int64_t)unit * a.R + r] : 0.0f;
+      st_lim = ok ? row_limit(a, n, row_query(a, r)) : 0;
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      *reinterpret_cast<u32x4v*>(&lds[buf][0][(tid + 256 * i) * 16]) = stage[0][i];
+      *reinterpret_cast<u32x4v*>(&lds[buf][1][(tid + 256 * i) * 16]) = stage[1][i];
+    }
+    if (tid < BM) row_lse[buf][tid] = st_lse, row_delta[buf][tid] = st_delta, row_lim[buf][tid] = st_lim;
+  };
+  if (r_begin < r_end) {
+    fetch(r_begin);
+    store(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int m0 = r_begin; m0 < r_end; m0 += BM, buf ^= 1) {
+    const bool more = m0 + BM < r_end;
+    if (more) fetch(m0 + BM);
+    const char *qt = lds[buf][0], *dot = lds[buf][1];
+    // rows see more keys the later they are: the tile needs no masks when its first row sees the wavefront's last key
+    const bool masked = m0 + BM > r_end || (a.causal && row_lim[buf][0] < tile * 128 + wave * 32 + 32);
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(qt, 32 * j + col, t, hi), kf[t], s);
+#pragma unroll
+      for (int t = 0; t < DK / 16; ++t) dp = mma(TL::row(dot, 32 * j + col, t, hi), vf[t], dp);
+      uint32_t w[4];
+      if (DROP) drop_words_keys(seed, (uint32_t)unit, m0 + 32 * j, key, lane, w);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int o = 32 * j + 8 * q + 4 * hi;
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_lse[buf][o]), delta = *reinterpret_cast<const f32x4*>(&row_delta[buf][o]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int g = 4 * q + c;
+          const bool see = !masked || key < row_lim[buf][o + c];
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse[c]));
+          const bool keep = !DROP || kept(w, g, a.thr);
+          const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
+          s[g] = see && keep ? p : 0.0f;
+          dp[g] = see ? p * (dpv - delta[c]) : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const Frag<T> p = acc_frag<T>(s, t), ds = acc_frag<T>(dp, t);
+#pragma unroll
+        for (int dt = 0; dt < DK / 32; ++dt) {
+          dv[dt] = mma(TL::col(dot, 32 * j + 16 * t, dt, lane), p, dv[dt]);
+          dk[dt] = mma(TL::col(qt, 32 * j + 16 * t, dt, lane), ds, dk[dt]);
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+  if (key >= a.Lk) return;
+  if (!live) {      // (a hidden key's column holds sums of no meaning, infinities among them: it is written as zeros)
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt) dk[dt] = f32x16{}, dv[dt] = f32x16{};
+  }
+  store_col<T, DK>(key_ptr<T>(a.dk, b, hk, key), a.D, hi, dk, a.scale);
+  store_col<T, DK>(key_ptr<T>(a.dv, b, hk, key), a.D, hi, dv, DROP ? a.keep_inv : 1.0f);
+}
+
+// ---- at most 32 keys: one wavefront per (sequence, key head), everything in one pass ------------------------------------
+// K and V stay in registers, rows come 32 at a time; delta is the row sum of P o m dP / keep, so that O is not read.
+template <typename T, int DK, bool DROP>
+__global__ __launch_bounds__(64, 1) void k_attn_bwd_short(Args a) {
+  constexpr int W = lds_width(DK);
+  typedef Tile<T, W> TL;
+  constexpr int kTileBytes = 32 * TL::kRowBytes, kPer = 32 * TL::kChunks / 64;
+  __shared__ __attribute__((aligned(16))) char lds[3][kTileBytes];      // K, Q, dO
+  __shared__ __attribute__((aligned(16))) float row_lse[32], row_delta[32];
+  __shared__ __attribute__((aligned(16))) int row_lim[32];
+  const int lane = threadIdx.x, hi = lane >> 5, col = lane & 31;
+  const int unit = (int)blockIdx.x, b = unit / a.Hk, hk = unit - b * a.Hk;
+  const Lens n = lens_of(a, b);
+  const int key = col;
+  const bool live = key < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + key] != 0);
+  const uint32_t vis = (uint32_t)__ballot(live);
+  const int r_end = n.q * a.G;
+  Frag<T> kf[DK / 16], vf[DK / 16];
+  load_row_frags<T, DK>(live ? key_ptr<T>(a.k, b, hk, key) : nullptr, live, a.D, hi, kf);
+  load_row_frags<T, DK>(live ? key_ptr<T>(a.v, b, hk, key) : nullptr, live, a.D, hi, vf);
+  auto put = [&](char* t, const Frag<T> (&f)[DK / 16]) {      // row fragments of 32 rows into an LDS tile
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<u32x4v*>(t + TL::chunk_off(col, 2 * i + hi)) = __builtin_bit_cast(u32x4v, f[i]);
+      } else {
+        *reinterpret_cast<f32x4*>(t + TL::chunk_off(col, 4 * i + 2 * hi)) = __builtin_shufflevector(f[i], f[i], 0, 1, 2, 3);
+        *reinterpret_cast<f32x4*>(t + TL::chunk_off(col, 4 * i + 2 * hi + 1)) = __builtin_shufflevector(f[i], f[i], 4, 5, 6, 7);
+      }
+    }
+  };
+  put(lds[0], kf);
+  f32x16 dk[DK / 32] = {}, dv[DK / 32] = {};
+  const uint64_t seed = DROP ? drop_seed(a) : 0;
+  for (int m0 = 0; m0 < a.R; m0 += 32) {
+    const int r = m0 + col, qi = row_query(a, r);
+    const bool row_ok = r < r_end;
+    const int lim = row_ok ? row_limit(a, n, qi) : 0;
+    const float lse2 = row_ok ? a.lse[(int64_t)unit * a.R + r] * kLog2e : 0.0f;
+    Frag<T> qf[DK / 16], dof[DK / 16];
+    load_row_frags<T, DK>(row_ok ? row_ptr<T>(a, a.q, b, hk, r) : nullptr, row_ok, a.D, hi, qf);
+    load_row_frags<T, DK>(row_ok ? row_ptr<T>(a, a.dout, b, hk, r) : nullptr, row_ok, a.D, hi, dof);
+    wave_lds_fence();
+    put(lds[1], qf);
+    put(lds[2], dof);
+    // rows in the lanes: delta, dQ
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) s = mma(kf[t], qf[t], s);
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) dp = mma(vf[t], dof[t], dp);
+    uint32_t w[4];
+    if (DROP) drop_words_rows(seed, (uint32_t)unit, r, 0, lane, w);
+    float delta = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) {
+      const int o = 8 * (g >> 2) + 4 * hi + (g & 3);
+      const bool see = o < lim && ((vis >> o) & 1);
+      const float p = see ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse2)) : 0.0f;
+      float dpv = see ? dp[g] : 0.0f;
+      if (DROP) dpv = kept(w, g, a.thr) ? dpv * a.keep_inv : 0.0f;
+      delta = __builtin_fmaf(p, dpv, delta);
+      s[g] = p, dp[g] = dpv;
+    }
+    delta = half_sum(delta);
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s[g] = s[g] * (dp[g] - delta);
+    if (hi == 0) row_lse[col] = lse2, row_delta[col] = delta, row_lim[col] = lim;
+    wave_lds_fence();
+    {
+      f32x16 dq[DK / 32] = {};
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const Frag<T> ds = acc_frag<T>(s, t);
+#pragma unroll
+        for (int dt = 0; dt < DK / 32; ++dt) dq[dt] = mma(TL::col(lds[0], 16 * t, dt, lane), ds, dq[dt]);
+      }
+      if (r < a.R) store_col<T, DK>(row_ptr<T>(a, a.dq, b, hk, r), a.D, hi, dq, row_ok ? a.scale : 0.0f);
+    }
+    // keys in the lanes: dK, dV
+    s = f32x16{}, dp = f32x16{};
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) s = mma(qf[t], kf[t], s);
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) dp = mma(dof[t], vf[t], dp);
+    if (DROP) drop_words_keys(seed, (uint32_t)unit, m0, key, lane, w);
+#pragma unroll
+    for (int g = 0; g < 16; ++g) {
+      const int o = 8 * (g >> 2) + 4 * hi + (g & 3);
+      const bool see = live && key < row_lim[o];
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -row_lse[o]));
+      const bool keep = !DROP || kept(w, g, a.thr);
+      const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
+      s[g] = see && keep ? p : 0.0f;
+      dp[g] = see ? p * (dpv - row_delta[o]) : 0.0f;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Frag<T> p = acc_frag<T>(s, t), ds = acc_frag<T>(dp, t);
+#pragma unroll
+      for (int dt = 0; dt < DK / 32; ++dt) {
+        dv[dt] = mma(TL::col(lds[2], 16 * t, dt, lane), p, dv[dt]);
+        dk[dt] = mma(TL::col(lds[1], 16 * t, dt, lane), ds, dk[dt]);
+      }
+    }
+  }
+  if (key >= a.Lk) return;
+  store_col<T, DK>(key_ptr<T>(a.dk, b, hk, key), a.D, hi, dk, a.scale);
+  store_col<T, DK>(key_ptr<T>(a.dv, b, hk, key), a.D, hi, dv, DROP ? a.keep_inv : 1.0f);
+}
+
+template <typename T, int DK, bool DROP>
+int launch(const Args& a0, hipStream_t st) {
+  Args a = a0;
+  const int64_t units = (int64_t)a.B * a.Hk;
+  if (a.Lk <= 32) {
+    if (units >= (1ll << 31)) return PSTL_ERR_SHAPE;
+    hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP>), dim3((unsigned)units), dim3(64), 0, st, a);
+    return launch_status();
+  }
+  if (a.R > 0) {
+    a.n_tiles = ceil_div(a.R, 128);
+    if (units * a.n_tiles >= (1ll << 31)) return PSTL_ERR_SHAPE;
+    hipLaunchKernelGGL((k_attn_bwd_q<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), 0, st, a);
+    if (int e = launch_status()) return e;
+  }
+  a.n_tiles = ceil_div(a.Lk, 128);
+  if (units * a.n_tiles >= (1ll << 31)) return PSTL_ERR_SHAPE;
+  hipLaunchKernelGGL((k_attn_bwd_kv<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), 0, st, a);
+  return launch_status();
+}
+template <typename T, int DK>
+int launch_drop(const Args& a, hipStream_t st) {
+  return a.thr ? launch<T, DK, true>(a, st) : launch<T, DK, false>(a, st);
+}
+template <typename T>
+int launch_dim(const Args& a, hipStream_t st) {
+  if (a.D <= 32) return launch_drop<T, 32>(a, st);
+  if (a.D <= 64) return launch_drop<T, 64>(a, st);
+  if (a.D <= 96) return launch_drop<T, 96>(a, st);
+  return launch_drop<T, 128>(a, st);
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace pstl
+
+using namespace pstl;
+using namespace pstl::attn;
+
+extern "C" size_t pstl_attention_backward_work_floats(const pstl_attn* c) {
+  Args a;
+  if (attn_args(c, &a, kCheckShape) != PSTL_OK) return 0;
+  return (size_t)a.B * a.Hk * a.R + 1;
+}
+
+extern "C" int pstl_attention_backward(const pstl_attn* c, void* stream) {
+  Args a;
+  if (int e = attn_args(c, &a, kCheckBackward)) return e;
+  if (a.B == 0 || (a.R == 0 && a.Lk == 0)) return PSTL_OK;
+  switch (c->dtype) {
+    case PSTL_F32: return launch_dim<float>(a, as_stream(stream));
+    case PSTL_BF16: return launch_dim<__bf16>(a, as_stream(stream));
+    default: return launch_dim<_Float16>(a, as_stream(stream));
+  }
+}

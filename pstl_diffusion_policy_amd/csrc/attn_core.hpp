@@ -1,0 +1,303 @@
+// attn_core.hpp -- building blocks of the attention kernels: element types, 32 x 32 matrix tiles, the swizzled LDS tile, packed
+// rows and the dropout decisions.
+//
+// Matrix tiles.  Every product is built from 32 x 32 accumulator tiles: lane l holds column l % 32, and register 4a + c (a, c in
+// 0..3) row 8a + 4 (l / 32) + c.  An operand fragment ("Frag") is eight values of the contraction index per lane: row (first
+// operand) or column (second operand) l % 32, slots 8 (l / 32) + j.  For 16-bit types one fragment pair is one
+// v_mfma_f32_32x32x16; for float32 the same fragments are eight v_mfma_f32_32x32x2 (slot j of both lane halves at a time), so
+// that both arithmetics share every layout.  A contraction over keys (or rows) pairs slots 0..3 with tile rows 4 (l / 32) + j and
+// slots 4..7 with 8 + 4 (l / 32) + j - 4: exactly the registers 8t .. 8t + 7 of an accumulator tile, which therefore become the
+// second operand of the next product without leaving the lane.
+//
+// Packed rows.  The G = Hq / Hk query heads that share a key head are rows of one matrix: row r = i G + g is query i of head
+// hk G + g.  Keys and values are then read once for all G heads, and the gradients of shared heads are sums inside one
+// accumulator, in a fixed order.
+#pragma once
+#include "pstl_common.hpp"
+#include "rng.hpp"
+
+namespace pstl {
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  typedef f32x8 x8;
+  typedef f32x4 x4;
+};
+template <>
+struct Vec<__bf16> {
+  typedef bf16x8 x8;
+  typedef bf16x4 x4;
+};
+template <>
+struct Vec<_Float16> {
+  typedef f16x8 x8;
+  typedef f16x4 x4;
+};
+template <typename T>
+using Frag = typename Vec<T>::x8;
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+__device__ inline f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ inline f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ inline f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// registers 8t .. 8t + 7 of an accumulator tile as an operand fragment (rounded to T: to nearest even)
+template <typename T>
+__device__ inline Frag<T> acc_frag(const f32x16& s, int t) {
+  f32x8 v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = s[8 * t + j];
+  return __builtin_convertvector(v, Frag<T>);
+}
+
+template <typename T>
+__device__ inline Frag<T> zero_frag() {
+  Frag<T> z;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z[j] = (T)0.0f;
+  return z;
+}
+
+// eight consecutive elements of global memory (16-byte aligned)
+template <typename T>
+__device__ inline Frag<T> load8(const T* p) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const u32x4v*>(p));
+  } else {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// this lane's value and the other lane half's: v_permlane32_swap_b32 exchanges the upper half of one register with the lower half
+// of another.  (The two operands are kept apart by an empty asm: with one value in both, the compiler names one register twice
+// and nothing is exchanged.)
+__device__ inline f32x2 both_halves(float x) {
+  uint32_t u = __builtin_bit_cast(uint32_t, x), v = u;
+  asm("" : "+v"(v));
+  const auto p = __builtin_amdgcn_permlane32_swap(u, v, false, false);
+  return f32x2{__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1])};
+}
+__device__ inline float half_max(float x) {
+  const f32x2 p = both_halves(x);
+  return fmaxf(p[0], p[1]);
+}
+__device__ inline float half_sum(float x) {
+  const f32x2 p = both_halves(x);
+  return p[0] + p[1];
+}
+
+// ---- LDS tiles ----------------------------------------------------------------------------------------------------
+// A tile of rows of W elements (a power of two) is stored row after row in 16-byte chunks; chunk c of row r sits at position
+// c ^ swz(r).  Rows 0..15 then put the same chunk on different banks (row fragments), and so do the four rows that a transposing
+// 16-bit read takes together (column fragments).
+template <typename T, int W>
+struct Tile {
+  static constexpr int kChunkEl = 16 / (int)sizeof(T);
+  static constexpr int kChunks = W / kChunkEl;
+  static constexpr int kRowBytes = W * (int)sizeof(T);
+  __device__ static inline int swz(int r) {
+    if constexpr (kChunks == 4) return (r >> 2) & 3;
+    if constexpr (kChunks == 8) return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+    return ((r & 7) << 1) | ((r >> 3) & 1);
+  }
+  __device__ static inline int chunk_off(int r, int c) { return r * kRowBytes + ((c ^ swz(r)) << 4); }
+  // row fragment: row `r`, elements 16 t + 8 hi + 0..7
+  __device__ static inline Frag<T> row(const char* lds, int r, int t, int hi) {
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const u32x4v*>(lds + chunk_off(r, 2 * t + hi)));
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + chunk_off(r, 4 * t + 2 * hi));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(lds + chunk_off(r, 4 * t + 2 * hi + 1));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // column fragment: element 32 dt + l % 32, slots = rows r0 + 4 hi + 0..3 and r0 + 8 + 4 hi + 0..3   (r0 a multiple of 16).
+  // 16-bit: ds_read_b64_tr_b16 hands lane i of a group of 16 the four rows' element i; lane i addresses row i / 4, elements
+  // 4 (i % 4) .. + 3.
+  __device__ static inline Frag<T> col(const char* lds, int r0, int dt, int lane) {
+    const int hi = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      typedef s16x4 __attribute__((address_space(3))) * lds_p;
+      const int i = lane & 15, d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+      const int r = r0 + 4 * hi + (i >> 2);
+      const char* p0 = lds + chunk_off(r, d >> 3) + (d & 7) * 2;
+      const char* p1 = lds + chunk_off(r + 8, d >> 3) + (d & 7) * 2;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p0);
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p1);
+      return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const int d = 32 * dt + (lane & 31);
+      Frag<T> v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = r0 + 4 * hi + (j & 3) + 8 * (j >> 2);
+        v[j] = *reinterpret_cast<const float*>(lds + chunk_off(r, d >> 2) + (d & 3) * 4);
+      }
+      return v;
+    }
+  }
+};
+
+// orders the LDS traffic of ONE wavefront (its instructions reach the LDS in order; this keeps the compiler to that order)
+__device__ inline void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// ---- dropout of probabilities ----------------------------------------------------------------------------------------
+// The decision for (row r, key j) of unit u = b Hk + hk is byte j % 4 of word r % 4 of philox(j / 4, r / 4, u, 'ATTD') under the
+// seed: a function of the element alone, whatever the kernel, tile or layout.  One draw serves a 4 x 4 patch, i.e. 16 elements
+// of 8 bits: with 16 bits per element the draws would be twice as many, and they are already a third of a training step's vector
+// work at D = 64; the probability is therefore a multiple of 1/256, and the scale is the inverse of the REALISED keep
+// probability.  A quad of lanes shares the four patches its 16 registers touch: lane i of the quad draws patch i, then the
+// words move across the quad by DPP -- one draw per lane and 32 x 32 tile in either layout.
+constexpr uint32_t kDropTag = 0x41545444u;
+
+template <int A>
+__device__ inline uint32_t quad_bcast(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, A * 0x55, 0xf, 0xf, true);
+}
+
+// lane = row r (any), registers = keys key0 + 8a + 4 hi + c (key0 a multiple of 32): W[a] = the four decision bytes of register
+// group a, key c in byte c
+__device__ inline void drop_words_rows(uint64_t seed, uint32_t unit, int r, int key0, int lane, uint32_t (&W)[4]) {
+  const uint32_t i = lane & 3, hi = lane >> 5;
+  const u32x4 w = philox4x32(u32x4{(uint32_t)(key0 >> 2) + 2 * i + hi, (uint32_t)(r >> 2), unit, kDropTag}, (uint32_t)seed,
+                             (uint32_t)(seed >> 32));
+  // W[a] = word i of lane a: a 4 x 4 transposition inside the quad
+#define PSTL_TR(A)                                                                                                \
+  {                                                                                                               \
+    const uint32_t x0 = quad_bcast<A>(w.x), x1 = quad_bcast<A>(w.y), x2 = quad_bcast<A>(w.z), x3 = quad_bcast<A>(w.w); \
+    const uint32_t lo = (i & 1) ? x1 : x0, up = (i & 1) ? x3 : x2;                                                \
+    W[A] = (i & 2) ? up : lo;                                                                                     \
+  }
+  PSTL_TR(0) PSTL_TR(1) PSTL_TR(2) PSTL_TR(3)
+#undef PSTL_TR
+}
+
+// lane = key, registers = rows row0 + 8a + 4 hi + c (row0 a multiple of 32): byte c of W[a] = the decision of row c of group a
+__device__ inline void drop_words_keys(uint64_t seed, uint32_t unit, int row0, int key, int lane, uint32_t (&W)[4]) {
+  const uint32_t i = lane & 3, hi = lane >> 5, sh = 8 * i;
+  const u32x4 w = philox4x32(u32x4{(uint32_t)(key >> 2), (uint32_t)(row0 >> 2) + 2 * i + hi, unit, kDropTag}, (uint32_t)seed,
+                             (uint32_t)(seed >> 32));
+#define PSTL_TR(A)                                                                                          \
+  W[A] = ((quad_bcast<A>(w.x) >> sh) & 255u) | (((quad_bcast<A>(w.y) >> sh) & 255u) << 8) |                 \
+         (((quad_bcast<A>(w.z) >> sh) & 255u) << 16) | (((quad_bcast<A>(w.w) >> sh) & 255u) << 24);
+  PSTL_TR(0) PSTL_TR(1) PSTL_TR(2) PSTL_TR(3)
+#undef PSTL_TR
+}
+__device__ inline bool kept(const uint32_t (&W)[4], int reg, uint32_t thr) {
+  return ((W[reg >> 2] >> (8 * (reg & 3))) & 255u) >= thr;
+}
+
+// ---- arguments -------------------------------------------------------------------------------------------------------
+struct Mat {      // (B, L, H, D), elements of a row consecutive; strides in elements
+  char* p;
+  int64_t sb, sl, sh;
+};
+struct Args {
+  Mat q, k, v, o, dout, dq, dk, dv;
+  float* lse;                 // (B, Hk, R): natural logarithm, -inf for a row that sees no key
+  float* delta;               // (B, Hk, R): sum_d dO O                      (backward's work)
+  const uint8_t* key_mask;    // (B, Lk), 0 = hidden, or null
+  int64_t mask_sb;
+  const int *q_lens, *k_lens; // (B) or null
+  float* part;                // (splits, units, rows, D) then (splits, units, rows, 2): partial results of a split call
+  const uint64_t* seed_dev;
+  uint64_t seed;
+  int B, Lq, Lk, Hk, G, D, R, causal;
+  uint32_t g_magic;           // r / G = umulhi(r, g_magic) for G > 1  (R G < 2^32, checked by the host)
+  float scale, c;             // c = scale log2(e)
+  uint32_t thr;               // a probability is dropped when its byte is below thr
+  float keep_inv;             // 256 / (256 - thr)
+  int n_tiles, splits, tiles_per_split;
+};
+
+__device__ inline int row_query(const Args& a, int r) { return a.G == 1 ? r : (int)__umulhi((uint32_t)r, a.g_magic); }
+__device__ inline uint64_t drop_seed(const Args& a) { return a.seed_dev ? uniform_u64(a.seed_dev) : a.seed; }
+
+// lengths of sequence b, clamped to the tensors
+struct Lens {
+  int q, k;
+};
+__device__ inline Lens lens_of(const Args& a, int b) {
+  Lens n;
+  n.q = a.q_lens ? min(max(__builtin_amdgcn_readfirstlane(a.q_lens[b]), 0), a.Lq) : a.Lq;
+  n.k = a.k_lens ? min(max(__builtin_amdgcn_readfirstlane(a.k_lens[b]), 0), a.Lk) : a.Lk;
+  return n;
+}
+// keys [0, limit) are what query i sees (before the key mask); causal masks are aligned to the sequences' ends
+__device__ inline int row_limit(const Args& a, Lens n, int i) {
+  if (i >= n.q) return 0;
+  if (!a.causal) return n.k;
+  return min(max(i + n.k - n.q + 1, 0), n.k);
+}
+template <typename T>
+__device__ inline T* row_ptr(const Args& a, const Mat& m, int b, int hk, int r) {
+  const int i = row_query(a, r), g = r - i * a.G;
+  return reinterpret_cast<T*>(m.p) + b * m.sb + i * m.sl + (int64_t)(hk * a.G + g) * m.sh;
+}
+template <typename T>
+__device__ inline T* key_ptr(const Mat& m, int b, int hk, int j) {
+  return reinterpret_cast<T*>(m.p) + b * m.sb + j * m.sl + hk * m.sh;
+}
+
+// workgroups are dealt to the 8 XCDs in turn: gives every XCD a consecutive share of [0, n), so that the workgroups that read the
+// same keys share one L2
+__device__ inline int xcd_order(int x, int n) {
+  const int q = n >> 3, rem = n & 7, xcd = x & 7;
+  return xcd * q + min(xcd, rem) + (x >> 3);
+}
+
+// row fragments of one packed row straight from global memory; zeros past D and for rows that are not there
+template <typename T, int DK>
+__device__ inline void load_row_frags(const T* p, bool ok, int D, int hi, Frag<T> (&f)[DK / 16]) {
+#pragma unroll
+  for (int t = 0; t < DK / 16; ++t) {
+    const int d = 16 * t + 8 * hi;
+    f[t] = (ok && d < D) ? load8<T>(p + d) : zero_frag<T>();
+  }
+}
+
+// stores an accumulator column (lane = row / key; registers = elements 32 dt + 8a + 4 hi + c) times `scale`
+template <typename T, int DK>
+__device__ inline void store_col(T* p, int D, int hi, const f32x16 (&acc)[DK / 32], float scale) {
+  typedef typename Vec<T>::x4 V4;
+#pragma unroll
+  for (int dt = 0; dt < DK / 32; ++dt) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int d = 32 * dt + 8 * a + 4 * hi;
+      f32x4 v;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = acc[dt][4 * a + c] * scale;
+      if (d < D) *reinterpret_cast<V4*>(p + d) = __builtin_convertvector(v, V4);
+    }
+  }
+}
+
+constexpr int lds_width(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
+
+}  // namespace attn
+}  // namespace pstl

@@ -26,7 +26,7 @@ HID = 256
 FEAT = 224
 NEI_PREP = 12
 
-ABI_VERSION = 6      # include/pstl_hip.h PSTL_ABI_VERSION
+ABI_VERSION = 7      # include/pstl_hip.h PSTL_ABI_VERSION
 SPLIT_F16_WMAX = 63.9   # include/pstl_hip.h PSTL_SPLIT_F16_WMAX
 ADAM_MAX_TENSORS = 32   # include/pstl_hip.h PSTL_ADAM_MAX_TENSORS
 
@@ -48,6 +48,28 @@ class Mlp3(ctypes.Structure):
 class WeightPtrs(ctypes.Structure):
     _fields_ = [(n, Mlp3) for n in ("ego_encoder", "neighbor_encoder", "lane_encoder", "policy_net", "merge_net",
                                     "rect_net")]
+
+
+class AttnMat(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_l", ctypes.c_int64), ("stride_h", ctypes.c_int64)]
+
+
+class QkRope(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "B", "L", "Hq", "Hk", "D", "rot", "interleaved")] +
+                [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)] +
+                [(n, AttnMat) for n in ("q", "k", "yq", "yk", "dyq", "dyk", "dq", "dk")] +
+                [("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                 ("pos_stride_b", ctypes.c_int64), ("inv_freq", ctypes.c_void_p), ("dwq", ctypes.c_void_p),
+                 ("dwk", ctypes.c_void_p), ("work", ctypes.c_void_p)])
+
+
+class Attn(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "B", "Lq", "Lk", "Hq", "Hk", "D", "causal")] +
+                [("scale", ctypes.c_float), ("dropout_256", ctypes.c_int32), ("seed", ctypes.c_uint64),
+                 ("seed_dev", ctypes.c_void_p)] +
+                [(n, AttnMat) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")] +
+                [("lse", ctypes.c_void_p), ("key_mask", ctypes.c_void_p), ("mask_stride_b", ctypes.c_int64),
+                 ("q_lens", ctypes.c_void_p), ("k_lens", ctypes.c_void_p), ("work", ctypes.c_void_p)])
 
 
 # One table for the exported symbols: (name, restype, argtypes).  `lib()` installs both, so that a wrong argument count or
@@ -96,6 +118,14 @@ SIGNATURES = [
     ("pstl_encoder_backward", _I, [_C] + [_P] * 17),
     ("pstl_merge_backward_work_floats", _Z, [_C]),
     ("pstl_merge_backward", _I, [_C, _P, _P, _P, _I] + [_P] * 8),
+    ("pstl_qk_norm_rope", _I, [_P, _P]),
+    ("pstl_qk_norm_rope_work_floats", _Z, [_P]),
+    ("pstl_qk_norm_rope_backward", _I, [_P, _P]),
+    ("pstl_attention_work_floats", _Z, [_P]),
+    ("pstl_attention", _I, [_P, _P]),
+    ("pstl_attention_backward_work_floats", _Z, [_P]),
+    ("pstl_attention_backward", _I, [_P, _P]),
+    ("pstl_dropout_add", _I, [_I, _L, _P, _P, _P, _I, _L, _P, _L, _P]),
 ]
 EXPORTS = sorted(set(n for n, _, _ in SIGNATURES))
 

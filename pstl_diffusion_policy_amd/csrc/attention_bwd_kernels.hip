@@ -251,66 +251,68 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_kv(
   store_col<T, DK>(key_ptr<T>(a.dv, b, hk, key), a.D, hi, dv, DROP ? a.keep_inv : 1.0f);
 }
 
-// ---- at most 32 keys: one wavefront per (sequence, key head), everything in one pass ------------------------------------
-// K and V stay in registers, rows come 32 at a time; delta is the row sum of P o m dP / keep, so that O is not read.
-template <typename T, int DK, bool DROP>
-__global__ __launch_bounds__(64, 1) void k_attn_bwd_short(Args a) {
-  constexpr int W = lds_width(DK);
-  typedef Tile<T, W> TL;
-  constexpr int kTileBytes = 32 * TL::kRowBytes, kPer = 32 * TL::kChunks / 64;
-  __shared__ __attribute__((aligned(16))) char lds[3][kTileBytes];      // K, Q, dO
-  __shared__ __attribute__((aligned(16))) float row_lse[32], row_delta[32];
-  __shared__ __attribute__((aligned(16))) int row_lim[32];
-  const int lane = threadIdx.x, hi = lane >> 5, col = lane & 31;
-  const int unit = (int)blockIdx.x, b = unit / a.Hk, hk = unit - b * a.Hk;
-  const Lens n = lens_of(a, b);
-  const int key = col;
-  const bool live = key < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + key] != 0);
-  const uint32_t vis = (uint32_t)__ballot(live);
-  const int r_end = n.q * a.G;
-  Frag<T> kf[DK / 16], vf[DK / 16];
-  load_row_frags<T, DK>(live ? key_ptr<T>(a.k, b, hk, key) : nullptr, live, a.D, hi, kf);
-  load_row_frags<T, DK>(live ? key_ptr<T>(a.v, b, hk, key) : nullptr, live, a.D, hi, vf);
-  auto put = [&](char* t, const Frag<T> (&f)[DK / 16]) {      // row fragments of 32 rows into an LDS tile
-#pragma unroll
-    for (int i = 0; i < DK / 16; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<u32x4v*>(t + TL::chunk_off(col, 2 * i + hi)) = __builtin_bit_cast(u32x4v, f[i]);
-      } else {
-        *reinterpret_cast<f32x4*>(t + TL::chunk_off(col, 4 * i + 2 * hi)) = __builtin_shufflevector(f[i], f[i], 0, 1, 2, 3);
-        *reinterpret_cast<f32x4*>(t + TL::chunk_off(col, 4 * i + 2 * hi + 1)) = __builtin_shufflevector(f[i], f[i], 4, 5, 6, 7);
-      }
-    }
+// ---- at most 32 keys: one wavefront per (sequence, key head), or per pair of them, everything in one pass ------------------
+// K and V stay in the LDS, rows come 32 at a time; delta is the row sum of P o m dP / keep, so that O is not read.  S and dP are
+// formed in both layouts (a product more against a transposition through the LDS).  Bound by memory, as the forward kernel.
+template <typename T, int DK, bool DROP, bool PAIR>
+__global__ __launch_bounds__(64 * (short_waves<T, DK>(4))) void k_attn_bwd_short(Args a) {
+  constexpr int NW = short_waves<T, DK>(4);
+  typedef Rows32<T, DK> RW;
+  constexpr int kTileBytes = 32 * RW::TL::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[NW][4][kTileBytes];
+  __shared__ __attribute__((aligned(16))) float row_stat[NW][2][32];
+  __shared__ __attribute__((aligned(16))) uint32_t row_see[NW][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, col = lane & 31;
+  const int units = a.B * a.Hk, u0 = ((int)blockIdx.x * NW + wave) * (PAIR ? 2 : 1);
+  if (u0 >= units) return;       // (no workgroup barrier below)
+  char *kt = lds[wave][0], *vt = lds[wave][1], *qt = lds[wave][2], *dot = lds[wave][3];
+  auto key_at = [&](const Mat& m) {
+    return [&, m](int row) -> T* {
+      const Slot s = slot_of<PAIR>(a, u0, units, row);
+      return s.ok && s.at < a.Lk ? key_ptr<T>(m, s.b, s.hk, s.at) : nullptr;
+    };
   };
-  put(lds[0], kf);
-  f32x16 dk[DK / 32] = {}, dv[DK / 32] = {};
+  RW kr, vr;
+  kr.load(key_at(a.k), a.D, lane);
+  vr.load(key_at(a.v), a.D, lane);
+  const Slot me = slot_of<PAIR>(a, u0, units, col);
+  const Lens n = lens_lane(a, me.b);
+  const bool key_on = me.ok && me.at < n.k && (!a.key_mask || a.key_mask[me.b * a.mask_sb + me.at] != 0);
+  const uint32_t keys_on = (uint32_t)__ballot(key_on);
   const uint64_t seed = DROP ? drop_seed(a) : 0;
+  f32x16 dk[DK / 32] = {}, dv[DK / 32] = {};
   for (int m0 = 0; m0 < a.R; m0 += 32) {
-    const int r = m0 + col, qi = row_query(a, r);
-    const bool row_ok = r < r_end;
-    const int lim = row_ok ? row_limit(a, n, qi) : 0;
-    const float lse2 = row_ok ? a.lse[(int64_t)unit * a.R + r] * kLog2e : 0.0f;
-    Frag<T> qf[DK / 16], dof[DK / 16];
-    load_row_frags<T, DK>(row_ok ? row_ptr<T>(a, a.q, b, hk, r) : nullptr, row_ok, a.D, hi, qf);
-    load_row_frags<T, DK>(row_ok ? row_ptr<T>(a, a.dout, b, hk, r) : nullptr, row_ok, a.D, hi, dof);
+    auto row_at = [&](const Mat& m) {
+      return [&, m](int row) -> T* {
+        const Slot s = slot_of<PAIR>(a, u0, units, row);
+        return s.ok && m0 + s.at < a.R ? row_ptr<T>(a, m, s.b, s.hk, m0 + s.at) : nullptr;
+      };
+    };
+    RW qr, dor;
+    qr.load(row_at(a.q), a.D, lane);
+    dor.load(row_at(a.dout), a.D, lane);
+    const int r = m0 + me.at, qi = row_query(a, r);
+    const bool live = me.ok && r < a.R && qi < n.q;
+    const uint32_t rows_on = (uint32_t)__ballot(live), see = seen_bits<PAIR>(keys_on, live ? row_limit(a, n, qi) : 0, lane);
+    const float lse2 = live ? a.lse[(int64_t)me.unit * a.R + r] * kLog2e : 0.0f;
     wave_lds_fence();
-    put(lds[1], qf);
-    put(lds[2], dof);
+    if (m0 == 0) {
+      kr.put(kt, keys_on, lane);
+      vr.put(vt, keys_on, lane);
+    }
+    qr.put(qt, rows_on, lane);
+    dor.put(dot, rows_on, lane);
+    wave_lds_fence();
     // rows in the lanes: delta, dQ
-    f32x16 s = {}, dp = {};
-#pragma unroll
-    for (int t = 0; t < DK / 16; ++t) s = mma(kf[t], qf[t], s);
-#pragma unroll
-    for (int t = 0; t < DK / 16; ++t) dp = mma(vf[t], dof[t], dp);
+    f32x16 s = row_product<T, DK>(kt, qt, lane), dp = row_product<T, DK>(vt, dot, lane);
     uint32_t w[4];
-    if (DROP) drop_words_rows(seed, (uint32_t)unit, r, 0, lane, w);
+    if (DROP) drop_words_rows<PAIR>(seed, (uint32_t)me.unit, r, 0, lane, w);
     float delta = 0.0f;
 #pragma unroll
     for (int g = 0; g < 16; ++g) {
-      const int o = 8 * (g >> 2) + 4 * hi + (g & 3);
-      const bool see = o < lim && ((vis >> o) & 1);
-      const float p = see ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse2)) : 0.0f;
-      float dpv = see ? dp[g] : 0.0f;
+      const bool on = ((see >> (4 * hi)) >> (8 * (g >> 2) + (g & 3))) & 1;
+      const float p = on ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse2)) : 0.0f;
+      float dpv = on ? dp[g] : 0.0f;
       if (DROP) dpv = kept(w, g, a.thr) ? dpv * a.keep_inv : 0.0f;
       delta = __builtin_fmaf(p, dpv, delta);
       s[g] = p, dp[g] = dpv;
@@ -318,48 +320,42 @@ __global__ __launch_bounds__(64, 1) void k_attn_bwd_short(Args a) {
     delta = half_sum(delta);
 #pragma unroll
     for (int g = 0; g < 16; ++g) s[g] = s[g] * (dp[g] - delta);
-    if (hi == 0) row_lse[col] = lse2, row_delta[col] = delta, row_lim[col] = lim;
+    if (hi == 0) row_stat[wave][0][col] = lse2, row_stat[wave][1][col] = delta, row_see[wave][col] = see;
+    f32x16 dq[DK / 32] = {};
+    contract<T, DK, PAIR>(dq, kt, s, lane);
     wave_lds_fence();
-    {
-      f32x16 dq[DK / 32] = {};
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const Frag<T> ds = acc_frag<T>(s, t);
-#pragma unroll
-        for (int dt = 0; dt < DK / 32; ++dt) dq[dt] = mma(TL::col(lds[0], 16 * t, dt, lane), ds, dq[dt]);
-      }
-      if (r < a.R) store_col<T, DK>(row_ptr<T>(a, a.dq, b, hk, r), a.D, hi, dq, row_ok ? a.scale : 0.0f);
-    }
     // keys in the lanes: dK, dV
-    s = f32x16{}, dp = f32x16{};
+    s = row_product<T, DK>(qt, kt, lane), dp = row_product<T, DK>(dot, vt, lane);
+    if (DROP) drop_words_keys<PAIR>(seed, (uint32_t)me.unit, m0, me.at, lane, w);
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t) s = mma(qf[t], kf[t], s);
+    for (int q = 0; q < 4; ++q) {
+      const int o = 8 * q + 4 * hi;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_stat[wave][0][o]), dl = *reinterpret_cast<const f32x4*>(&row_stat[wave][1][o]);
+      const u32x4v sees = *reinterpret_cast<const u32x4v*>(&row_see[wave][o]);
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t) dp = mma(dof[t], vf[t], dp);
-    if (DROP) drop_words_keys(seed, (uint32_t)unit, m0, key, lane, w);
-#pragma unroll
-    for (int g = 0; g < 16; ++g) {
-      const int o = 8 * (g >> 2) + 4 * hi + (g & 3);
-      const bool see = live && key < row_lim[o];
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -row_lse[o]));
-      const bool keep = !DROP || kept(w, g, a.thr);
-      const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
-      s[g] = see && keep ? p : 0.0f;
-      dp[g] = see ? p * (dpv - row_delta[o]) : 0.0f;
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Frag<T> p = acc_frag<T>(s, t), ds = acc_frag<T>(dp, t);
-#pragma unroll
-      for (int dt = 0; dt < DK / 32; ++dt) {
-        dv[dt] = mma(TL::col(lds[2], 16 * t, dt, lane), p, dv[dt]);
-        dk[dt] = mma(TL::col(lds[1], 16 * t, dt, lane), ds, dk[dt]);
+      for (int c = 0; c < 4; ++c) {
+        const int g = 4 * q + c;
+        const bool on = (sees[c] >> col) & 1;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse[c]));
+        const bool keep = !DROP || kept(w, g, a.thr);
+        const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
+        s[g] = on && keep ? p : 0.0f;
+        dp[g] = on ? p * (dpv - dl[c]) : 0.0f;
       }
     }
+    contract<T, DK, PAIR>(dv, dot, s, lane);
+    contract<T, DK, PAIR>(dk, qt, dp, lane);
+    wave_lds_fence();
+    RW::from_acc(qt, col, hi, dq, a.scale, live);
+    wave_lds_fence();
+    RW::store(qt, row_at(a.dq), a.D, lane);
   }
-  if (key >= a.Lk) return;
-  store_col<T, DK>(key_ptr<T>(a.dk, b, hk, key), a.D, hi, dk, a.scale);
-  store_col<T, DK>(key_ptr<T>(a.dv, b, hk, key), a.D, hi, dv, DROP ? a.keep_inv : 1.0f);
+  wave_lds_fence();
+  RW::from_acc(kt, col, hi, dk, a.scale, key_on);
+  RW::from_acc(vt, col, hi, dv, DROP ? a.keep_inv : 1.0f, key_on);
+  wave_lds_fence();
+  RW::store(kt, key_at(a.dk), a.D, lane);
+  RW::store(vt, key_at(a.dv), a.D, lane);
 }
 
 template <typename T, int DK, bool DROP>
@@ -367,8 +363,14 @@ int launch(const Args& a0, hipStream_t st) {
   Args a = a0;
   const int64_t units = (int64_t)a.B * a.Hk;
   if (a.Lk <= 32) {
-    if (units >= (1ll << 31)) return PSTL_ERR_SHAPE;
-    hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP>), dim3((unsigned)units), dim3(64), 0, st, a);
+    constexpr int NW = short_waves<T, DK>(4);
+    const bool pair = in_pairs(a);
+    const int64_t jobs = pair ? (units + 1) / 2 : units;
+    const dim3 grid((unsigned)((jobs + NW - 1) / NW)), block(64 * NW);
+    if (pair)
+      hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, true>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, false>), grid, block, 0, st, a);
     return launch_status();
   }
   if (a.R > 0) {

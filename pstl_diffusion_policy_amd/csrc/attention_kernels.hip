@@ -144,28 +144,98 @@ __global__ __launch_bounds__(256, 2) void k_attn_fwd(Args a) {
   store_col<T, DK>(row_ptr<T>(a, a.o, b, hk, r), a.D, hi, acc, live ? inv : 0.0f);
 }
 
-// ---- few rows: 32 packed rows; every wavefront walks keys of its own ----------------------------------------------------
-// SPLIT: the four wavefronts of a workgroup (and `splits` workgroups) share one set of rows and divide its keys; their results
-// are joined in the LDS (and by k_attn_join).  Otherwise every wavefront has rows of its own (many short sequences).
-// Keys go straight to the matrix operands; values pass through the wavefront's own LDS tile to be read by columns.
-template <typename T, int DK, bool DROP, bool SPLIT>
+// ---- at most 32 keys: one wavefront per 32 packed rows, or per pair of units of at most 16 rows and keys -----------------
+// Bound by memory: q, k and v pass through the wavefront's LDS tiles and o leaves the same way, so that neighbouring lanes touch
+// neighbouring 16 bytes (fragments read straight from global memory touch 32 rows per instruction: 82 us instead of the 59 us of
+// this kernel at 4096 x 12 tokens, 8 heads of 32, float32).
+template <typename T, int DK, bool DROP, bool PAIR>
+__global__ __launch_bounds__(64 * (short_waves<T, DK>(3))) void k_attn_fwd_short(Args a) {
+  constexpr int NW = short_waves<T, DK>(3);
+  typedef Rows32<T, DK> RW;
+  constexpr int kTileBytes = 32 * RW::TL::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[NW][3][kTileBytes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, col = lane & 31;
+  const int units = a.B * a.Hk, groups = PAIR ? (units + 1) / 2 : units;
+  const int job = (int)blockIdx.x * NW + wave;
+  if (job >= groups * a.n_tiles) return;       // (no workgroup barrier below)
+  const int group = job / a.n_tiles, tile = job - group * a.n_tiles, u0 = PAIR ? 2 * group : group;
+  char *kt = lds[wave][0], *vt = lds[wave][1], *qt = lds[wave][2];
+  // (loads are bounded by the tensors, not by the lengths and masks, so that they do not wait for those)
+  RW kr, vr, qr;
+  auto key_at = [&](const Mat& m) {
+    return [&, m](int row) -> const T* {
+      const Slot s = slot_of<PAIR>(a, u0, units, row);
+      return s.ok && s.at < a.Lk ? key_ptr<T>(m, s.b, s.hk, s.at) : nullptr;
+    };
+  };
+  auto row_at = [&](const Mat& m) {
+    return [&, m](int row) -> T* {
+      const Slot s = slot_of<PAIR>(a, u0, units, row);
+      const int r = tile * 32 + s.at;
+      return s.ok && r < a.R ? row_ptr<T>(a, m, s.b, s.hk, r) : nullptr;
+    };
+  };
+  kr.load(key_at(a.k), a.D, lane);
+  qr.load(row_at(a.q), a.D, lane);
+  vr.load(key_at(a.v), a.D, lane);
+  const Slot me = slot_of<PAIR>(a, u0, units, col);
+  const Lens n = lens_lane(a, me.b);
+  const int r = tile * 32 + me.at, qi = row_query(a, r);
+  const bool key_on = me.ok && me.at < n.k && (!a.key_mask || a.key_mask[me.b * a.mask_sb + me.at] != 0);
+  const bool live = me.ok && r < a.R && qi < n.q;
+  const uint32_t keys_on = (uint32_t)__ballot(key_on), rows_on = (uint32_t)__ballot(live);
+  const uint32_t see = seen_bits<PAIR>(keys_on, live ? row_limit(a, n, qi) : 0, lane) >> (4 * hi);
+  kr.put(kt, keys_on, lane);
+  qr.put(qt, rows_on, lane);
+  vr.put(vt, keys_on, lane);
+  wave_lds_fence();
+  f32x16 s = row_product<T, DK>(kt, qt, lane);
+  float mx = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < 16; ++g) {
+    s[g] = (see >> (8 * (g >> 2) + (g & 3))) & 1 ? s[g] : -INFINITY;
+    mx = fmaxf(mx, s[g]);
+  }
+  const float m = half_max(mx) * a.c, mu = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+#pragma unroll
+  for (int g = 0; g < 16; ++g) {
+    s[g] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -mu));
+    l += s[g];
+  }
+  l = half_sum(l);
+  if (DROP) {
+    uint32_t w[4];
+    drop_words_rows<PAIR>(drop_seed(a), (uint32_t)me.unit, r, 0, lane, w);
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s[g] = kept(w, g, a.thr) ? s[g] : 0.0f;
+  }
+  f32x16 acc[DK / 32] = {};
+  contract<T, DK, PAIR>(acc, vt, s, lane);
+  const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : l;      // (0 for a row that sees nothing; a NaN sum stays one)
+  if (hi == 0 && a.lse && me.ok && r < a.R)
+    a.lse[(int64_t)me.unit * a.R + r] = live && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  wave_lds_fence();
+  RW::from_acc(qt, col, hi, acc, inv, live);
+  wave_lds_fence();
+  RW::store(qt, row_at(a.o), a.D, lane);
+}
+
+// ---- few rows, many keys: 32 packed rows; every wavefront walks keys of its own ------------------------------------------
+// The four wavefronts of a workgroup (and `splits` workgroups) share one set of rows and divide its keys; their results are
+// joined in the LDS (and by k_attn_join).  Bound by reading the keys and values once: tiles of 32 keys are fetched a tile ahead
+// into registers, 16 bytes per lane along the rows, and pass through the wavefront's own LDS tiles.
+template <typename T, int DK, bool DROP>
 __global__ __launch_bounds__(256) void k_attn_fwd_few(Args a) {
-  constexpr int W = lds_width(DK);
-  typedef Tile<T, W> TL;
-  constexpr int kTileBytes = 32 * TL::kRowBytes, kPer = 32 * TL::kChunks / 64;
-  constexpr int kJoinBytes = SPLIT ? 32 * DK * 4 : 0, kWaveBytes = kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes;
-  __shared__ __attribute__((aligned(16))) char lds[4][kWaveBytes];
+  typedef Rows32<T, DK> RW;
+  typedef typename RW::TL TL;
+  constexpr int kTileBytes = 32 * TL::kRowBytes;
+  constexpr int kJoinBytes = 32 * DK * 4, kWaveBytes = 2 * kTileBytes > kJoinBytes ? 2 * kTileBytes : kJoinBytes;
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // 4 x kWaveBytes
   __shared__ float stat[4][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, col = lane & 31;
-  const int jobs = a.B * a.Hk * a.n_tiles;
-  int job, split = 0;
-  if (SPLIT) {
-    const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
-    job = work / a.splits, split = work - job * a.splits;
-  } else {
-    job = (int)blockIdx.x * 4 + wave;
-    if (job >= jobs) return;       // (no workgroup barrier below in this form)
-  }
+  const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const int job = work / a.splits, split = work - job * a.splits;
   const int unit = job / a.n_tiles, tile = job - unit * a.n_tiles;
   const int b = unit / a.Hk, hk = unit - b * a.Hk;
   const Lens n = lens_of(a, b);
@@ -174,41 +244,39 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(Args a) {
   const int lim = live ? row_limit(a, n, qi) : 0;
   const int q_first = row_query(a, tile * 32), q_last = min(row_query(a, min(tile * 32 + 31, a.R - 1)), n.q - 1);
   const int kall = q_first < n.q ? row_limit(a, n, q_last) : 0;
-  const int t_lo = SPLIT ? split * a.tiles_per_split + wave : 0, t_step = SPLIT ? 4 : 1;
-  const int kend = SPLIT ? min(kall, (split + 1) * a.tiles_per_split * 32) : kall;
+  const int k_lo = (split * a.tiles_per_split + wave) * 32, kend = min(kall, (split + 1) * a.tiles_per_split * 32);
 
   Frag<T> qf[DK / 16];
   load_row_frags<T, DK>(live ? row_ptr<T>(a, a.q, b, hk, r) : nullptr, live, a.D, hi, qf);
   f32x16 acc[DK / 32] = {};
   float m = -INFINITY, l = 0.0f;
   const uint64_t seed = DROP ? drop_seed(a) : 0;
-  char* vt = lds[wave];
-  for (int k0 = t_lo * 32; k0 < kend; k0 += 32 * t_step) {
-    const int key = k0 + col;
-    const bool key_ok = key < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + key] != 0);
-    const uint32_t vis = (uint32_t)__ballot(key_ok);
-    Frag<T> kf[DK / 16];
-    load_row_frags<T, DK>(key_ok ? key_ptr<T>(a.k, b, hk, key) : nullptr, key_ok, a.D, hi, kf);
-    u32x4v stage[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int id = lane + 64 * i, row = id / TL::kChunks, d = ((id % TL::kChunks) ^ TL::swz(row)) * TL::kChunkEl;
-      const bool ok = ((vis >> row) & 1) && d < a.D;
-      stage[i] = ok ? *reinterpret_cast<const u32x4v*>(key_ptr<T>(a.v, b, hk, k0 + row) + d) : u32x4v{0, 0, 0, 0};
-    }
+  char *kt = lds + wave * kWaveBytes, *vt = kt + kTileBytes;
+  RW kr, vr;
+  uint32_t vis = 0;
+  auto fetch = [&](int k0) {
+    auto at = [&](const Mat& mt) {
+      return [&, mt](int row) -> const T* { return k0 + row < n.k ? key_ptr<T>(mt, b, hk, k0 + row) : nullptr; };
+    };
+    kr.load(at(a.k), a.D, lane);
+    vr.load(at(a.v), a.D, lane);
+    vis = (uint32_t)__ballot(k0 + col < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + k0 + col] != 0));
+  };
+  if (k_lo < kend) fetch(k_lo);
+  for (int k0 = k_lo; k0 < kend; k0 += 128) {
     wave_lds_fence();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) *reinterpret_cast<u32x4v*>(vt + (lane + 64 * i) * 16) = stage[i];
+    kr.put(kt, vis, lane);
+    vr.put(vt, vis, lane);
+    const uint32_t see = seen_bits<false>(vis, min(max(lim - k0, 0), 32), lane) >> (4 * hi);
+    if (k0 + 128 < kend) fetch(k0 + 128);
     wave_lds_fence();
     f32x16 s = {};
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t) s = mma(kf[t], qf[t], s);
+    for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(kt, col, t, hi), qf[t], s);
     float mx = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 16; ++g) {
-      const int o = 8 * (g >> 2) + 4 * hi + (g & 3);
-      const bool see = k0 + o < lim && ((vis >> o) & 1);
-      s[g] = see ? s[g] : -INFINITY;
+      s[g] = (see >> (8 * (g >> 2) + (g & 3))) & 1 ? s[g] : -INFINITY;
       mx = fmaxf(mx, s[g]);
     }
     const float m_new = fmaxf(m, half_max(mx) * a.c), mu = m_new == -INFINITY ? 0.0f : m_new;
@@ -231,91 +299,109 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(Args a) {
     for (int dt = 0; dt < DK / 32; ++dt)
 #pragma unroll
       for (int g = 0; g < 16; ++g) acc[dt][g] *= alpha;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Frag<T> p = acc_frag<T>(s, t);
-#pragma unroll
-      for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = mma(TL::col(vt, 16 * t, dt, lane), p, acc[dt]);
-    }
+    contract<T, DK, false>(acc, vt, s, lane);
   }
   l = half_sum(l);
-  if constexpr (!SPLIT) {
-    if (r >= a.R) return;
-    const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : (l == 0.0f ? 0.0f : l);
-    if (hi == 0 && a.lse) a.lse[(int64_t)unit * a.R + r] = live && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
-    store_col<T, DK>(row_ptr<T>(a, a.o, b, hk, r), a.D, hi, acc, live ? inv : 0.0f);
-  } else {
-    // join the wavefronts: common maximum, then the sum of the rescaled parts in the fixed order 0..3
-    if (hi == 0) stat[wave][0][col] = m;
-    __syncthreads();
-    const float mj = fmaxf(fmaxf(stat[0][0][col], stat[1][0][col]), fmaxf(stat[2][0][col], stat[3][0][col]));
-    const float f = __builtin_amdgcn_exp2f(m - (mj == -INFINITY ? 0.0f : mj));
-    if (hi == 0) stat[wave][1][col] = l * f;
-    float* part = reinterpret_cast<float*>(lds[wave]);
+  // join the wavefronts: common maximum, then the sum of the rescaled parts in the fixed order 0..3
+  if (hi == 0) stat[wave][0][col] = m;
+  __syncthreads();
+  const float mj = fmaxf(fmaxf(stat[0][0][col], stat[1][0][col]), fmaxf(stat[2][0][col], stat[3][0][col]));
+  const float f = __builtin_amdgcn_exp2f(m - (mj == -INFINITY ? 0.0f : mj));
+  if (hi == 0) stat[wave][1][col] = l * f;
+  float* part = reinterpret_cast<float*>(lds + wave * kWaveBytes);
 #pragma unroll
-    for (int dt = 0; dt < DK / 32; ++dt)
+  for (int dt = 0; dt < DK / 32; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 v;
+    for (int g = 0; g < 4; ++g) {
+      f32x4 v;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = acc[dt][4 * g + c] * f;
-        *reinterpret_cast<f32x4*>(part + col * DK + 32 * dt + 8 * g + 4 * hi) = v;
+      for (int c = 0; c < 4; ++c) v[c] = acc[dt][4 * g + c] * f;
+      *reinterpret_cast<f32x4*>(part + col * DK + 32 * dt + 8 * g + 4 * hi) = v;
+    }
+  __syncthreads();
+  for (int e = tid; e < 32 * (DK / 4); e += 256) {
+    const int row = e / (DK / 4), d = (e - row * (DK / 4)) * 4, rr = tile * 32 + row;
+    if (rr >= a.R || d >= a.D) continue;
+    f32x4 v = {};
+    float ls = 0.0f, mr = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * kWaveBytes) + row * DK + d);
+      ls += stat[w][1][row];
+      mr = fmaxf(mr, stat[w][0][row]);
+    }
+    if (a.splits > 1) {
+      const int64_t units = (int64_t)a.B * a.Hk, at = ((int64_t)split * units + unit) * a.R + rr;
+      *reinterpret_cast<f32x4*>(a.part + at * a.D + d) = v;
+      if (d == 0) {
+        float* st = a.part + (int64_t)a.splits * units * a.R * a.D + 2 * at;
+        st[0] = mr, st[1] = ls;
       }
-    __syncthreads();
-    for (int e = tid; e < 32 * (DK / 4); e += 256) {
-      const int row = e / (DK / 4), d = (e - row * (DK / 4)) * 4, rr = tile * 32 + row;
-      if (rr >= a.R || d >= a.D) continue;
-      f32x4 v = {};
-      float ls = 0.0f, mr = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) + row * DK + d);
-        ls += stat[w][1][row];
-        mr = fmaxf(mr, stat[w][0][row]);
-      }
-      if (a.splits > 1) {
-        const int64_t units = (int64_t)a.B * a.Hk, at = ((int64_t)split * units + unit) * a.R + rr;
-        *reinterpret_cast<f32x4*>(a.part + at * a.D + d) = v;
-        if (d == 0) {
-          float* st = a.part + (int64_t)a.splits * units * a.R * a.D + 2 * at;
-          st[0] = mr, st[1] = ls;
-        }
-      } else {
-        const bool lv = row_query(a, rr) < n.q;
-        const float inv = lv ? (ls > 0.0f ? (DROP ? a.keep_inv : 1.0f) / ls : (ls == 0.0f ? 0.0f : ls)) : 0.0f;
-        typedef typename Vec<T>::x4 V4;
-        *reinterpret_cast<V4*>(row_ptr<T>(a, a.o, b, hk, rr) + d) = __builtin_convertvector(v * inv, V4);
-        if (d == 0 && a.lse)
-          a.lse[(int64_t)unit * a.R + rr] = lv && ls != 0.0f ? (mr + __builtin_amdgcn_logf(ls)) * kLn2 : -INFINITY;
-      }
+    } else {
+      const bool lv = row_query(a, rr) < n.q;
+      const float inv = ls > 0.0f ? (DROP ? a.keep_inv : 1.0f) / ls : ls;
+      typedef typename Vec<T>::x4 V4;
+      v = lv ? v * inv : f32x4{};
+      *reinterpret_cast<V4*>(row_ptr<T>(a, a.o, b, hk, rr) + d) = __builtin_convertvector(v, V4);
+      if (d == 0 && a.lse) a.lse[(int64_t)unit * a.R + rr] = lv && ls != 0.0f ? (mr + __builtin_amdgcn_logf(ls)) * kLn2 : -INFINITY;
     }
   }
 }
 
-// joins the parts of a split call: thread = (row, four elements)
+// joins the parts of a split call: one workgroup per row; eight groups of 32 lanes (four elements each) sum every eighth part,
+// and the groups' sums are joined in order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(Args a, float gain) {
-  const int per = a.D / 4;
-  const int64_t units = (int64_t)a.B * a.Hk, rows = units * a.R, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= rows * per) return;
-  const int64_t row = e / per;
-  const int d = (int)(e - row * per) * 4, unit = (int)(row / a.R), r = (int)(row - (int64_t)unit * a.R);
-  const int b = unit / a.Hk, hk = unit - b * a.Hk;
+  __shared__ float weight[kMaxSplits], red[8];
+  __shared__ f32x4 sums[8][32];
+  const int tid = threadIdx.x, lane = tid & 31, g = tid >> 5;
+  const int64_t rows = (int64_t)a.B * a.Hk * a.R, row = blockIdx.x;
+  const int unit = (int)(row / a.R), r = (int)(row - (int64_t)unit * a.R), b = unit / a.Hk, hk = unit - b * a.Hk;
   const float* st = a.part + (int64_t)a.splits * rows * a.D;
   float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, st[2 * (s * rows + row)]);
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
-  f32x4 v = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(st[2 * (s * rows + row)] - mu);
-    l += f * st[2 * (s * rows + row) + 1];
-    v += f * *reinterpret_cast<const f32x4*>(a.part + (s * rows + row) * a.D + d);
+  for (int s = tid; s < a.splits; s += 256) {
+    const float x = st[2 * (s * rows + row)];
+    weight[s] = x;
+    m = fmaxf(m, x);
   }
-  const float inv = l > 0.0f ? gain / l : (l == 0.0f ? 0.0f : l);
-  typedef typename Vec<T>::x4 V4;
-  *reinterpret_cast<V4*>(row_ptr<T>(a, a.o, b, hk, r) + d) = __builtin_convertvector(v * inv, V4);
-  if (d == 0 && a.lse) a.lse[row] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (lane == 0) red[g] = m;
+  __syncthreads();
+  m = red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
+  const float mu = m == -INFINITY ? 0.0f : m;
+  __syncthreads();
+  float l = 0.0f;
+  for (int s = tid; s < a.splits; s += 256) {
+    const float f = __builtin_amdgcn_exp2f(weight[s] - mu);
+    weight[s] = f;
+    l += f * st[2 * (s * rows + row) + 1];
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) l += __shfl_xor(l, o);
+  if (lane == 0) red[g] = l;
+  __syncthreads();
+  f32x4 v = {};
+  const int d = 4 * lane;
+  if (d < a.D) {
+#pragma unroll 4
+    for (int s = g; s < a.splits; s += 8) v += weight[s] * *reinterpret_cast<const f32x4*>(a.part + (s * rows + row) * a.D + d);
+  }
+  sums[g][lane] = v;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) l += red[i];
+  if (g == 0 && d < a.D) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += sums[i][lane];
+    const float inv = l > 0.0f ? gain / l : (l == 0.0f ? 0.0f : l);
+    typedef typename Vec<T>::x4 V4;
+    *reinterpret_cast<V4*>(row_ptr<T>(a, a.o, b, hk, r) + d) = __builtin_convertvector(v * inv, V4);
+  }
+  if (tid == 0 && a.lse) a.lse[row] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
 template <typename T, int DK, bool DROP>
@@ -325,14 +411,29 @@ int launch(const Args& a0, const FwdPlan& p, hipStream_t st) {
   const int64_t units = (int64_t)a.B * a.Hk;
   if (p.kind == kManyRows) {
     hipLaunchKernelGGL((k_attn_fwd<T, DK, DROP>), dim3((unsigned)(units * p.n_tiles)), dim3(256), 0, st, a);
-  } else if (p.kind == kFewRowsOwn) {
-    hipLaunchKernelGGL((k_attn_fwd_few<T, DK, DROP, false>), dim3((unsigned)((units * p.n_tiles + 3) / 4)), dim3(256), 0, st, a);
+  } else if (p.kind == kShort || p.kind == kShortPairs) {
+    constexpr int NW = short_waves<T, DK>(3);
+    const bool pair = p.kind == kShortPairs;
+    const int64_t jobs = (pair ? (units + 1) / 2 : units) * p.n_tiles;
+    const dim3 grid((unsigned)((jobs + NW - 1) / NW)), block(64 * NW);
+    if (pair)
+      hipLaunchKernelGGL((k_attn_fwd_short<T, DK, DROP, true>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((k_attn_fwd_short<T, DK, DROP, false>), grid, block, 0, st, a);
   } else {
-    hipLaunchKernelGGL((k_attn_fwd_few<T, DK, DROP, true>), dim3((unsigned)(units * p.n_tiles * p.splits)), dim3(256), 0, st, a);
+    constexpr int kTile2 = 2 * 32 * lds_width(DK) * (int)sizeof(T), kJoin = 32 * DK * 4, kBytes = 4 * (kTile2 > kJoin ? kTile2 : kJoin);
+    static DeviceOnce once;
+    const int dev = current_device();
+    if (!once.done(dev)) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_fwd_few<T, DK, DROP>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              kBytes) != hipSuccess)
+        return PSTL_ERR_LAUNCH;
+      once.set(dev);
+    }
+    hipLaunchKernelGGL((k_attn_fwd_few<T, DK, DROP>), dim3((unsigned)(units * p.n_tiles * p.splits)), dim3(256), kBytes, st, a);
     if (p.splits > 1) {
       if (int e = launch_status()) return e;
-      const int64_t n = units * a.R * (a.D / 4);
-      hipLaunchKernelGGL((k_attn_join<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, DROP ? a.keep_inv : 1.0f);
+      hipLaunchKernelGGL((k_attn_join<T>), dim3((unsigned)(units * a.R)), dim3(256), 0, st, a, DROP ? a.keep_inv : 1.0f);
     }
   }
   return launch_status();

@@ -180,10 +180,11 @@ __device__ inline uint32_t quad_bcast(uint32_t x) {
 }
 
 // lane = row r (any), registers = keys key0 + 8a + 4 hi + c (key0 a multiple of 32): W[a] = the four decision bytes of register
-// group a, key c in byte c
+// group a, key c in byte c.  PAIR: the tile holds two units of 16 keys (groups 0, 1 and 2, 3), `unit` and r are the lane's own.
+template <bool PAIR = false>
 __device__ inline void drop_words_rows(uint64_t seed, uint32_t unit, int r, int key0, int lane, uint32_t (&W)[4]) {
   const uint32_t i = lane & 3, hi = lane >> 5;
-  const u32x4 w = philox4x32(u32x4{(uint32_t)(key0 >> 2) + 2 * i + hi, (uint32_t)(r >> 2), unit, kDropTag}, (uint32_t)seed,
+  const u32x4 w = philox4x32(u32x4{(uint32_t)(key0 >> 2) + 2 * (PAIR ? i & 1 : i) + hi, (uint32_t)(r >> 2), unit, kDropTag}, (uint32_t)seed,
                              (uint32_t)(seed >> 32));
   // W[a] = word i of lane a: a 4 x 4 transposition inside the quad
 #define PSTL_TR(A)                                                                                                \
@@ -197,9 +198,10 @@ __device__ inline void drop_words_rows(uint64_t seed, uint32_t unit, int r, int 
 }
 
 // lane = key, registers = rows row0 + 8a + 4 hi + c (row0 a multiple of 32): byte c of W[a] = the decision of row c of group a
+template <bool PAIR = false>
 __device__ inline void drop_words_keys(uint64_t seed, uint32_t unit, int row0, int key, int lane, uint32_t (&W)[4]) {
   const uint32_t i = lane & 3, hi = lane >> 5, sh = 8 * i;
-  const u32x4 w = philox4x32(u32x4{(uint32_t)(key >> 2), (uint32_t)(row0 >> 2) + 2 * i + hi, unit, kDropTag}, (uint32_t)seed,
+  const u32x4 w = philox4x32(u32x4{(uint32_t)(key >> 2), (uint32_t)(row0 >> 2) + 2 * (PAIR ? i & 1 : i) + hi, unit, kDropTag}, (uint32_t)seed,
                              (uint32_t)(seed >> 32));
 #define PSTL_TR(A)                                                                                          \
   W[A] = ((quad_bcast<A>(w.x) >> sh) & 255u) | (((quad_bcast<A>(w.y) >> sh) & 255u) << 8) |                 \
@@ -228,6 +230,7 @@ struct Args {
   uint64_t seed;
   int B, Lq, Lk, Hk, G, D, R, causal;
   uint32_t g_magic;           // r / G = umulhi(r, g_magic) for G > 1  (R G < 2^32, checked by the host)
+  uint32_t hk_magic;          // unit / Hk likewise, where a kernel divides lane by lane (short sequences in pairs)
   float scale, c;             // c = scale log2(e)
   uint32_t thr;               // a probability is dropped when its byte is below thr
   float keep_inv;             // 256 / (256 - thr)
@@ -298,6 +301,121 @@ __device__ inline void store_col(T* p, int D, int hi, const f32x16 (&acc)[DK / 3
 }
 
 constexpr int lds_width(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
+
+// ---- short sequences: 32 packed rows and 32 keys, one wavefront ---------------------------------------------------------
+// PAIR: two units (sequence, key head) of at most 16 rows and 16 keys share a wavefront: rows and keys 0..15 are the first's,
+// 16..31 the second's.  A score between the two is masked away, and their sums never meet: the contraction over the first
+// sixteen slots belongs to the first unit, the other sixteen to the second, each with an accumulator of its own (0 * NaN is NaN,
+// and one unit's NaN must not reach its neighbour).
+struct Slot {        // what a row of the tile stands for
+  int unit, b, hk, at;
+  bool ok;
+};
+template <bool PAIR>
+__device__ inline Slot slot_of(const Args& a, int first_unit, int units, int row) {
+  Slot s;
+  s.unit = PAIR ? first_unit + (row >> 4) : first_unit;
+  s.at = PAIR ? row & 15 : row;
+  s.ok = s.unit < units;
+  const int u = s.ok ? s.unit : first_unit;
+  s.b = PAIR ? (a.Hk == 1 ? u : (int)__umulhi((uint32_t)u, a.hk_magic)) : u / a.Hk;
+  s.hk = u - s.b * a.Hk;
+  return s;
+}
+__device__ inline Lens lens_lane(const Args& a, int b) {
+  Lens n;
+  n.q = a.q_lens ? min(max(a.q_lens[b], 0), a.Lq) : a.Lq;
+  n.k = a.k_lens ? min(max(a.k_lens[b], 0), a.Lk) : a.Lk;
+  return n;
+}
+// 32 rows of global memory to / from an LDS tile, 16 bytes per lane, neighbouring lanes on neighbouring chunks
+template <typename T, int DK>
+struct Rows32 {
+  typedef Tile<T, lds_width(DK)> TL;
+  static constexpr int kPer = 32 * TL::kChunks / 64;
+  u32x4v v[kPer];
+  template <typename F>
+  __device__ inline void load(F ptr, int D, int lane) {      // ptr(row) -> the row's first element, or null
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = lane + 64 * i, row = id / TL::kChunks, d = ((id % TL::kChunks) ^ TL::swz(row)) * TL::kChunkEl;
+      const T* p = ptr(row);
+      v[i] = p && d < D ? *reinterpret_cast<const u32x4v*>(p + d) : u32x4v{0, 0, 0, 0};
+    }
+  }
+  __device__ inline void put(char* tile, uint32_t rows_on, int lane) const {      // rows that are off: zeros
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = lane + 64 * i, row = id / TL::kChunks;
+      *reinterpret_cast<u32x4v*>(tile + id * 16) = (rows_on >> row) & 1 ? v[i] : u32x4v{0, 0, 0, 0};
+    }
+  }
+  template <typename F>
+  __device__ static inline void store(const char* tile, F ptr, int D, int lane) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = lane + 64 * i, row = id / TL::kChunks, d = ((id % TL::kChunks) ^ TL::swz(row)) * TL::kChunkEl;
+      T* p = ptr(row);
+      if (p && d < D) *reinterpret_cast<u32x4v*>(p + d) = *reinterpret_cast<const u32x4v*>(tile + id * 16);
+    }
+  }
+  // an accumulator column (lane = row) into the tile's row
+  __device__ static inline void from_acc(char* tile, int row, int hi, const f32x16 (&acc)[DK / 32], float scale, bool on) {
+    typedef typename Vec<T>::x4 V4;
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 x;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = on ? acc[dt][4 * g + c] * scale : 0.0f;
+        const int d = 32 * dt + 8 * g + 4 * hi;
+        *reinterpret_cast<V4*>(tile + TL::chunk_off(row, d / TL::kChunkEl) + (d % TL::kChunkEl) * (int)sizeof(T)) =
+            __builtin_convertvector(x, V4);
+      }
+  }
+};
+// sum over the tile's 32 slots of  A(slot) x f(slot):  acc[dt] (+)= columns of `tile` times the fragments of s; PAIR: the lane's half
+template <typename T, int DK, bool PAIR>
+__device__ inline void contract(f32x16 (&acc)[DK / 32], const char* tile, const f32x16& s, int lane) {
+  typedef Tile<T, lds_width(DK)> TL;
+  const Frag<T> f0 = acc_frag<T>(s, 0), f1 = acc_frag<T>(s, 1);
+  const bool second = (lane & 16) != 0;
+#pragma unroll
+  for (int dt = 0; dt < DK / 32; ++dt) {
+    if constexpr (PAIR) {
+      const f32x16 x0 = mma(TL::col(tile, 0, dt, lane), f0, acc[dt]), x1 = mma(TL::col(tile, 16, dt, lane), f1, acc[dt]);
+#pragma unroll
+      for (int g = 0; g < 16; ++g) acc[dt][g] = second ? x1[g] : x0[g];
+    } else {
+      acc[dt] = mma(TL::col(tile, 0, dt, lane), f0, acc[dt]);
+      acc[dt] = mma(TL::col(tile, 16, dt, lane), f1, acc[dt]);
+    }
+  }
+}
+// the tile's product over the element index: result(row i of x, lane = row of y)
+template <typename T, int DK>
+__device__ inline f32x16 row_product(const char* x, const char* y, int lane) {
+  typedef Tile<T, lds_width(DK)> TL;
+  f32x16 s = {};
+#pragma unroll
+  for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(x, lane & 31, t, lane >> 5), TL::row(y, lane & 31, t, lane >> 5), s);
+  return s;
+}
+// the keys of the tile that this lane's row sees, as bits (lim: its first `lim` keys)
+template <bool PAIR>
+__device__ inline uint32_t seen_bits(uint32_t keys_on, int lim, int lane) {
+  if constexpr (PAIR) {
+    const uint32_t own = (1u << min(lim, 16)) - 1u;
+    return keys_on & (own << (lane & 16));
+  } else {
+    return keys_on & (lim >= 32 ? ~0u : (1u << lim) - 1u);
+  }
+}
+template <typename T, int DK>
+constexpr int short_waves(int tiles) {      // wavefronts (each with its own tiles) per workgroup
+  return tiles * 32 * lds_width(DK) * (int)sizeof(T) <= 16384 ? 4 : tiles * 32 * lds_width(DK) * (int)sizeof(T) <= 32768 ? 2 : 1;
+}
 
 }  // namespace attn
 }  // namespace pstl

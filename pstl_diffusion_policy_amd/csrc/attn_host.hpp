@@ -35,6 +35,7 @@ inline int attn_args(const pstl_attn* c, Args* a, Check what) {
   a->part = c->work, a->delta = c->work, a->seed = c->seed, a->seed_dev = c->seed_dev;
   a->B = c->B, a->Lq = c->Lq, a->Lk = c->Lk, a->Hk = c->Hk, a->G = (int)G, a->D = c->D, a->R = (int)R, a->causal = c->causal != 0;
   a->g_magic = G > 1 ? (uint32_t)((1ull << 32) / (uint64_t)G + 1) : 0;
+  a->hk_magic = c->Hk > 1 ? (uint32_t)((1ull << 32) / (uint64_t)c->Hk + 1) : 0;
   a->scale = c->scale, a->c = c->scale * kLog2e;
   a->thr = (uint32_t)thr, a->keep_inv = 256.0f / (float)(256 - thr);
   if (what == kCheckShape) return PSTL_OK;
@@ -51,29 +52,35 @@ inline int attn_args(const pstl_attn* c, Args* a, Check what) {
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
-enum Kind { kManyRows, kFewRowsOwn, kFewRowsSplit };
+constexpr int kMaxSplits = 1024;
+enum Kind { kManyRows, kShort, kShortPairs, kFewRows };
 struct FwdPlan {
   Kind kind;
   int n_tiles, splits, tiles_per_split;
 };
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// two units share a wavefront (attn_core.hpp, Slot)
+inline bool in_pairs(const Args& a) {
+  return a.Lk <= 16 && a.R <= 16 && (int64_t)a.B * a.Hk * a.Hk < (1ll << 31);
+}
 inline FwdPlan plan_forward(const Args& a, int cus) {
   const int64_t units = (int64_t)a.B * a.Hk;
   FwdPlan p = {kManyRows, ceil_div(a.R, 128), 1, 0};
-  const bool few = a.R <= 32 || a.Lk <= 64 || (units * p.n_tiles * 2 < cus && a.R <= 256 && a.Lk >= 1024);
-  if (!few) return p;
-  p.n_tiles = ceil_div(a.R, 32);
-  const int64_t jobs = units * p.n_tiles;
-  const int key_tiles = ceil_div(a.Lk, 32);
-  if (key_tiles <= 1 || jobs >= 8 * cus) {
-    p.kind = kFewRowsOwn;
+  if (a.Lk <= 32) {
+    p.kind = in_pairs(a) ? kShortPairs : kShort;
+    p.n_tiles = ceil_div(a.R, 32);
     return p;
   }
-  p.kind = kFewRowsSplit;
-  const int64_t want = (2 * cus + jobs - 1) / jobs;
-  const int most = ceil_div(key_tiles, 4);
+  const bool few = a.R <= 32 || (units * p.n_tiles * 2 < cus && a.R <= 256 && a.Lk >= 1024);
+  if (!few) return p;
+  p.kind = kFewRows;
+  p.n_tiles = ceil_div(a.R, 32);
+  const int64_t jobs = units * p.n_tiles;
+  const int key_tiles = ceil_div(a.Lk, 32), most = ceil_div(key_tiles, 4);
+  const int64_t want = jobs >= cus ? 1 : (2 * cus + jobs - 1) / jobs;
   p.splits = (int)(want < most ? want : most);
+  if (p.splits > kMaxSplits) p.splits = kMaxSplits;
   p.tiles_per_split = ceil_div(ceil_div(key_tiles, p.splits), 4) * 4;
   p.splits = ceil_div(key_tiles, p.tiles_per_split);
   return p;

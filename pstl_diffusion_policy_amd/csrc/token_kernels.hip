@@ -158,19 +158,27 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs p) {
   }
 }
 
-// dw[s][d] = sum over the workgroups' parts: one workgroup per (s, 32 elements), eight strided sums each, joined in order
-__global__ __launch_bounds__(256) void k_qk_norm_rope_dw(const float* part, int blocks, int D, float* dwq, float* dwk) {
-  __shared__ float s[8][32];
+// dw[s][d] = sum over the workgroups' parts: one workgroup per (s, 32 elements), 32 strided sums each, joined in order.  Bound by
+// the latency of its loads: eight are in flight per thread (8 strided sums with one load in flight took 60 us for 2048 parts).
+__global__ __launch_bounds__(1024) void k_qk_norm_rope_dw(const float* part, int blocks, int D, float* dwq, float* dwk) {
+  __shared__ float s[32][32];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, d = (int)blockIdx.x * 32 + lane, which = blockIdx.y;
   float sum = 0.0f;
-  if (d < D)
-    for (int i = g; i < blocks; i += 8) sum += part[((int64_t)i * 2 + which) * D + d];
+  if (d < D) {
+    for (int i0 = g; i0 < blocks; i0 += 256) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i0 + 32 * u < blocks ? part[((int64_t)(i0 + 32 * u) * 2 + which) * D + d] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += v[u];
+    }
+  }
   s[g][lane] = sum;
   __syncthreads();
   if (g == 0 && d < D) {
     float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += s[i][lane];
+    for (int i = 0; i < 32; ++i) v += s[i][lane];
     (which ? dwk : dwq)[d] = v;
   }
 }
@@ -295,7 +303,7 @@ int rope_launch(RopeArgs& p, bool backward, float* dwq, float* dwk, hipStream_t 
     if (int e = launch_status()) return e;
   }
   if (backward)
-    hipLaunchKernelGGL(k_qk_norm_rope_dw, dim3((p.D + 31) / 32, 2), dim3(256), 0, st, p.part, blocks, p.D, dwq, dwk);
+    hipLaunchKernelGGL(k_qk_norm_rope_dw, dim3((p.D + 31) / 32, 2), dim3(1024), 0, st, p.part, blocks, p.D, dwq, dwk);
   return launch_status();
 }
 int rope_run(const pstl_qk_rope* c, bool backward, void* stream) {

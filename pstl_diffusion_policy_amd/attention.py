@@ -18,8 +18,8 @@ engine.DynBlock): a captured step draws another mask at each replay.  It must ke
 
 There is no CPU path: tensors must live on the GPU and the library must be built (ffi.lib() raises otherwise).
 """
-import ctypes
 import math
+import struct
 
 import torch
 
@@ -28,7 +28,11 @@ from . import ffi
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_HEAD_DIM = 128            # attention (include/pstl_hip.h, PSTL_ATTN_MAX_D)
 MAX_ROPE_HEAD_DIM = 256       # qk_norm_rope (PSTL_ROPE_MAX_D)
-_NO_MAT = (None, 0, 0, 0)
+_NO_MAT = (0, 0, 0, 0)
+# pstl_attn and pstl_qk_rope as bytes (ffi.Attn, ffi.QkRope; a ctypes.Structure takes longer to fill than a small call runs)
+_ATTN = struct.Struct("@8ifiQQ32q6q")
+_ROPE = struct.Struct("@8ifi32q8q")
+_raw_stream = torch._C._cuda_getCurrentRawStream      # current_stream().cuda_stream without the two objects around it
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -43,7 +47,7 @@ def _rows(name, t, like=None):
     if t.dim() != 4:
         raise ValueError("%s must be (B, L, H, D), got %s" % (name, tuple(t.shape)))
     if like is not None:
-        if t.dtype != like.dtype:
+        if t.dtype is not like.dtype:
             raise TypeError("%s is %s, the queries are %s" % (name, t.dtype, like.dtype))
         if t.device != like.device:
             raise ValueError("%s is on %s, the queries are on %s" % (name, t.device, like.device))
@@ -69,10 +73,11 @@ def _check_aligned(name, t):
 
 
 def _mat(t):
-    if t is None:
-        return _NO_MAT
-    sb, sl, sh, _ = t.stride()
-    return (t.data_ptr(), sb, sl, sh)
+    return (t.data_ptr(),) + t.stride()[:3]
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _gradient(t, like):
@@ -113,6 +118,16 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
+def _once(backward):
+    """torch.autograd.function.once_differentiable (a second derivative raises), entered only when a graph of the backward pass is
+    asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
 
@@ -127,7 +142,9 @@ def rope_frequencies(rot_dim, base=10000.0, device=None):
     return float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
 
 
-def _rope_checks(q, k, q_weight, k_weight, positions, inv_freq):
+def _rope_checks(q, k, q_weight, k_weight, positions, inv_freq, eps):
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative, got %r" % (eps,))
     _rows("q", q)
     _rows("k", k, q)
     B, L, Hq, D = q.shape
@@ -159,56 +176,63 @@ def _rope_checks(q, k, q_weight, k_weight, positions, inv_freq):
             raise ValueError("%s must be 16-byte aligned" % name)
 
 
-def _rope_struct(q, k, wq, wk, positions, inv_freq, eps, interleaved, yq=None, yk=None, dyq=None, dyk=None, dq=None, dk=None,
-                 dwq=None, dwk=None, work=None):
+def _rope_launch(q, k, wq, wk, positions, inv_freq, eps, interleaved, grads=None):
+    """The call on checked operands; grads = (dyq, dyk): the backward pass."""
     B, L, Hq, D = q.shape
-    p = lambda t: None if t is None else t.data_ptr()
-    return ffi.QkRope(_CODES[q.dtype], B, L, Hq, k.shape[2], D, 2 * inv_freq.numel(), int(bool(interleaved)), eps, 0, _mat(q),
-                      _mat(k), _mat(yq), _mat(yk), _mat(dyq), _mat(dyk), _mat(dq), _mat(dk), wq.data_ptr(), wk.data_ptr(),
-                      positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0, inv_freq.data_ptr(), p(dwq),
-                      p(dwk), p(work))
+    dev = q.device
+    with _on_device(dev):
+        yq, yk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))      # forward's results, or the gradients of q and k
+        if grads is None:
+            mats, tail = _mat(yq) + _mat(yk) + 4 * _NO_MAT, (0, 0, 0)
+        else:
+            dyq, dyk = _gradient(grads[0], q), _gradient(grads[1], k)
+            dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+            mats = 2 * _NO_MAT + _mat(dyq) + _mat(dyk) + _mat(yq) + _mat(yk)
+            tail = (dwq.data_ptr(), dwk.data_ptr(), 0)
+        head = (_CODES[q.dtype], B, L, Hq, k.shape[2], D, 2 * inv_freq.numel(), 1 if interleaved else 0, eps, 0) + _mat(q) + _mat(k)
+        mid = (wq.data_ptr(), wk.data_ptr(), positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
+               inv_freq.data_ptr())
+        lib = ffi.lib()
+        a = _ROPE.pack(*head, *mats, *mid, *tail)
+        if grads is None:
+            rc = lib.pstl_qk_norm_rope(a, _raw_stream(dev.index))
+            if rc:
+                ffi.check(rc, "qk_norm_rope")
+            return yq, yk
+        work = torch.empty(lib.pstl_qk_norm_rope_work_floats(a), dtype=torch.float32, device=dev)
+        rc = lib.pstl_qk_norm_rope_backward(_ROPE.pack(*head, *mats, *mid, *tail[:2], work.data_ptr()), _raw_stream(dev.index))
+        if rc:
+            ffi.check(rc, "qk_norm_rope_backward")
+        return yq, yk, dwq, dwk
 
 
 def qk_norm_rope_forward(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """qk_norm_rope without autograd."""
-    _rope_checks(q, k, q_weight, k_weight, positions, inv_freq)
-    with _on_device(q.device):
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        a = _rope_struct(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, yq, yk)
-        ffi.check(ffi.lib().pstl_qk_norm_rope(ctypes.byref(a), ffi.stream()), "qk_norm_rope")
-    return yq, yk
+    _rope_checks(q, k, q_weight, k_weight, positions, inv_freq, eps)
+    return _rope_launch(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
 
 
 def qk_norm_rope_backward(dyq, dyk, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """(dq, dk, dq_weight, dk_weight) of qk_norm_rope, from its ORIGINAL inputs and the gradients of its outputs."""
-    _rope_checks(q, k, q_weight, k_weight, positions, inv_freq)
+    _rope_checks(q, k, q_weight, k_weight, positions, inv_freq, eps)
     for name, t, x in (("dyq", dyq, q), ("dyk", dyk, k)):
         if t.shape != x.shape or t.device != x.device:
             raise ValueError("%s must be %s on %s" % (name, tuple(x.shape), x.device))
-    with _on_device(q.device):
-        dyq, dyk = _gradient(dyq, q), _gradient(dyk, k)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
-        a = _rope_struct(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, None, None, dyq, dyk, dq, dk, dwq, dwk)
-        work = torch.empty(ffi.lib().pstl_qk_norm_rope_work_floats(ctypes.byref(a)), dtype=torch.float32, device=q.device)
-        a.work = work.data_ptr()
-        ffi.check(ffi.lib().pstl_qk_norm_rope_backward(ctypes.byref(a), ffi.stream()), "qk_norm_rope_backward")
-    return dq, dk, dwq, dwk
+    return _rope_launch(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, (dyq, dyk))
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, positions, inv_freq, eps, interleaved):
+        _rope_checks(q, k, wq, wk, positions, inv_freq, eps)
         ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
         ctx.opts = (eps, interleaved)
-        return qk_norm_rope_forward(q, k, wq, wk, positions, inv_freq, eps, interleaved)
+        return _rope_launch(q, k, wq, wk, positions, inv_freq, eps, interleaved)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dyq, dyk):
-        return qk_norm_rope_backward(dyq, dyk, *ctx.saved_tensors, *ctx.opts) + (None,) * 4
+        return _rope_launch(*ctx.saved_tensors, *ctx.opts, (dyq, dyk)) + (None,) * 4
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
@@ -272,13 +296,45 @@ def _attn_scale(scale, D):
     return scale
 
 
-def _attn_struct(q, k, v, o, causal, scale, n256, seed, seed_dev, key_mask, q_lens, k_lens, lse=None, dout=None, dq=None,
-                 dk=None, dv=None):
+def _attn_forward(q, k, v, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev, need_lse):
+    """The call on checked operands: (out, lse or None)."""
     B, Lq, Hq, D = q.shape
-    p = lambda t: None if t is None else t.data_ptr()
-    return ffi.Attn(_CODES[q.dtype], B, Lq, k.shape[1], Hq, k.shape[2], D, int(bool(causal)), scale, n256, seed, p(seed_dev),
-                    _mat(q), _mat(k), _mat(v), _mat(o), _mat(dout), _mat(dq), _mat(dk), _mat(dv), p(lse), p(key_mask),
-                    0 if key_mask is None else key_mask.stride(0), p(q_lens), p(k_lens), None)
+    Lk, Hk = k.shape[1], k.shape[2]
+    dev = q.device
+    with _on_device(dev):
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        lse = torch.empty((B, Hk, Lq, Hq // Hk), dtype=torch.float32, device=dev) if need_lse else None
+        head = (_CODES[q.dtype], B, Lq, Lk, Hq, Hk, D, 1 if causal else 0, scale, n256, seed, _ptr(seed_dev)) + _mat(q) + _mat(k) \
+            + _mat(v) + _mat(out) + 4 * _NO_MAT
+        tail = (_ptr(lse), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _ptr(q_lens), _ptr(k_lens))
+        lib = ffi.lib()
+        a = _ATTN.pack(*head, *tail, 0)
+        n = lib.pstl_attention_work_floats(a) if Lk > 32 else 0      # (a split call: few rows, many keys)
+        if n:
+            work = torch.empty(n, dtype=torch.float32, device=dev)
+            a = _ATTN.pack(*head, *tail, work.data_ptr())
+        rc = lib.pstl_attention(a, _raw_stream(dev.index))
+        if rc:
+            ffi.check(rc, "attention")
+    return out, lse
+
+
+def _attn_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev):
+    """The call on checked operands: (dq, dk, dv)."""
+    B, Lq, Hq, D = q.shape
+    dev = q.device
+    with _on_device(dev):
+        dout = _gradient(dout, q)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        head = (_CODES[q.dtype], B, Lq, k.shape[1], Hq, k.shape[2], D, 1 if causal else 0, scale, n256, seed, _ptr(seed_dev)) \
+            + _mat(q) + _mat(k) + _mat(v) + _mat(out) + _mat(dout) + _mat(dq) + _mat(dk) + _mat(dv) \
+            + (lse.data_ptr(), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _ptr(q_lens), _ptr(k_lens))
+        lib = ffi.lib()
+        work = torch.empty(lib.pstl_attention_backward_work_floats(_ATTN.pack(*head, 0)), dtype=torch.float32, device=dev)
+        rc = lib.pstl_attention_backward(_ATTN.pack(*head, work.data_ptr()), _raw_stream(dev.index))
+        if rc:
+            ffi.check(rc, "attention_backward")
+    return dq, dk, dv
 
 
 def attention_forward(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, scale=None, dropout_p=0.0, seed=0,
@@ -286,30 +342,14 @@ def attention_forward(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=
     """attention without autograd: (out, lse).  lse (B, Hk, Lq, Hq/Hk) float32 is what attention_backward takes (None with
     need_lse=False)."""
     n256 = _attn_checks(q, k, v, key_mask, q_lens, k_lens, dropout_p)
-    scale = _attn_scale(scale, q.shape[3])
-    seed, seed_dev = _seed(seed, q.device)
-    B, Lq, Hq, _ = q.shape
-    Hk = k.shape[2]
-    with _on_device(q.device):
-        L = ffi.lib()
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((B, Hk, Lq, Hq // Hk), dtype=torch.float32, device=q.device) if need_lse else None
-        a = _attn_struct(q, k, v, out, causal, scale, n256, seed, seed_dev, key_mask, q_lens, k_lens, lse)
-        ref = ctypes.byref(a)
-        n = L.pstl_attention_work_floats(ref)
-        if n:
-            work = torch.empty(n, dtype=torch.float32, device=q.device)
-            a.work = work.data_ptr()
-        ffi.check(L.pstl_attention(ref, ffi.stream()), "attention")
-    return out, lse
+    return _attn_forward(q, k, v, causal, key_mask, q_lens, k_lens, _attn_scale(scale, q.shape[3]), n256, *_seed(seed, q.device),
+                         need_lse)
 
 
 def attention_backward(dout, q, k, v, out, lse, causal=False, key_mask=None, q_lens=None, k_lens=None, scale=None,
                        dropout_p=0.0, seed=0):
     """(dq, dk, dv) of attention, from its inputs, its results and the gradient of `out`.  Deterministic: no atomics."""
     n256 = _attn_checks(q, k, v, key_mask, q_lens, k_lens, dropout_p)
-    scale = _attn_scale(scale, q.shape[3])
-    seed, seed_dev = _seed(seed, q.device)
     B, Lq, Hq, _ = q.shape
     Hk = k.shape[2]
     for name, t in (("dout", dout), ("out", out)):
@@ -319,39 +359,31 @@ def attention_backward(dout, q, k, v, out, lse, causal=False, key_mask=None, q_l
             or lse.device != q.device):
         raise ValueError("out (%s) and lse (float32, %s) are what attention_forward returned" % (q.dtype, (B, Hk, Lq, Hq // Hk)))
     _check_aligned("out", out)
-    with _on_device(q.device):
-        L = ffi.lib()
-        dout = _gradient(dout, q)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        a = _attn_struct(q, k, v, out, causal, scale, n256, seed, seed_dev, key_mask, q_lens, k_lens, lse, dout, dq, dk, dv)
-        ref = ctypes.byref(a)
-        work = torch.empty(L.pstl_attention_backward_work_floats(ref), dtype=torch.float32, device=q.device)
-        a.work = work.data_ptr()
-        ffi.check(L.pstl_attention_backward(ref, ffi.stream()), "attention_backward")
-    return dq, dk, dv
+    return _attn_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, _attn_scale(scale, q.shape[3]), n256,
+                          *_seed(seed, q.device))
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed):
-        out, lse = attention_forward(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed)
-        on_device = isinstance(seed, torch.Tensor)
+    def forward(ctx, q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed, want_lse):
+        n256 = _attn_checks(q, k, v, key_mask, q_lens, k_lens, dropout_p)
+        scale = _attn_scale(scale, q.shape[3])
+        seed, seed_dev = _seed(seed, q.device)
+        out, lse = _attn_forward(q, k, v, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev, True)
         # (saved, so that autograd refuses a backward pass whose masks, lengths or seed were overwritten in between)
-        ctx.save_for_backward(q, k, v, out, lse, key_mask, q_lens, k_lens, seed if on_device else None)
-        ctx.opts = (causal, scale, dropout_p, None if on_device else seed)
+        ctx.save_for_backward(q, k, v, out, lse, key_mask, q_lens, k_lens, seed_dev)
+        ctx.opts = (causal, scale, n256, seed)
+        if not want_lse:
+            return out
         ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
-        if dout is None:
-            return (None,) * 10
+    @_once
+    def backward(ctx, dout, *_):
         q, k, v, out, lse, key_mask, q_lens, k_lens, seed_dev = ctx.saved_tensors
-        causal, scale, dropout_p, seed = ctx.opts
-        return attention_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, scale, dropout_p,
-                                  seed if seed_dev is None else seed_dev) + (None,) * 7
+        causal, scale, n256, seed = ctx.opts
+        return _attn_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev) + (None,) * 8
 
 
 def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, scale=None, dropout_p=0.0, seed=0,
@@ -369,11 +401,14 @@ def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, sc
     draws the mask.  return_lse: also the log of the softmax's sums, (B, Hq, Lq) float32, without a gradient.
     Differentiable in q, k and v; the backward pass forms the probabilities again and is deterministic."""
     if _needs_grad(q, k, v):
-        out, lse = _Attention.apply(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed)
+        res = _Attention.apply(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed, return_lse)
+        if not return_lse:
+            return res
+        out, lse = res
     else:
         out, lse = attention_forward(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed, need_lse=return_lse)
-    if not return_lse:
-        return out
+        if not return_lse:
+            return out
     B, Lq, Hq, _ = q.shape
     return out, lse.permute(0, 1, 3, 2).reshape(B, Hq, Lq)
 
@@ -381,17 +416,18 @@ def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, sc
 # ---------------------------------------------------------------------------------------------------------------
 # dropout
 # ---------------------------------------------------------------------------------------------------------------
-def _dropout_launch(x, residual, p, seed, offset):
-    value, seed_dev = _seed(seed, x.device)
-    _on_gpu(x)
-    with _on_device(x.device):
-        x = x.contiguous()
-        residual = None if residual is None else residual.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        q = lambda t: None if t is None else t.data_ptr()
-        ffi.check(ffi.lib().pstl_dropout_add(_CODES[x.dtype], x.numel(), x.data_ptr(), q(residual), y.data_ptr(),
-                                             int(round(65536 * p)), value - 2 ** 64 if value >= 2 ** 63 else value, q(seed_dev),
-                                             offset, ffi.stream()), "dropout_add")
+def _dropout_launch(x, residual, p, value, seed_dev, offset):
+    dev = x.device
+    with _on_device(dev):
+        if not x.is_contiguous():
+            x = x.contiguous()
+        if residual is not None and not residual.is_contiguous():
+            residual = residual.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        rc = ffi.lib().pstl_dropout_add(_CODES[x.dtype], x.numel(), x.data_ptr(), _ptr(residual), y.data_ptr(), int(round(65536 * p)),
+                                        value - 2 ** 64 if value >= 2 ** 63 else value, _ptr(seed_dev), offset, _raw_stream(dev.index))
+        if rc:
+            ffi.check(rc, "dropout_add")
     return y
 
 
@@ -412,24 +448,25 @@ def _dropout_checks(x, p, offset, residual):
 def dropout_backward(dy, p, seed, offset=0):
     """The gradient of dropout_add in x: the same mask on dy (its gradient in the residual is dy itself)."""
     _dropout_checks(dy, p, offset, None)
-    return _dropout_launch(dy, None, p, seed, offset)
+    seed = _seed(seed, dy.device)
+    _on_gpu(dy)
+    return _dropout_launch(dy, None, p, *seed, offset)
 
 
 class _DropoutAdd(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        on_device = isinstance(seed, torch.Tensor)
-        ctx.save_for_backward(seed if on_device else None)
-        ctx.opts = (p, None if on_device else seed, offset)
-        return _dropout_launch(x, residual, p, seed, offset)
+    def forward(ctx, x, residual, p, seed, seed_dev, offset):
+        ctx.save_for_backward(seed_dev)
+        ctx.opts = (p, seed, offset)
+        return _dropout_launch(x, residual, p, seed, seed_dev, offset)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         p, seed, offset = ctx.opts
-        seed_dev, = ctx.saved_tensors
-        dx = _dropout_launch(dy, None, p, seed if seed_dev is None else seed_dev, offset) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        need_x, need_residual = ctx.needs_input_grad[:2]
+        dx = _dropout_launch(dy, None, p, seed, ctx.saved_tensors[0], offset) if need_x else None
+        return dx, dy if need_residual else None, None, None, None, None
 
 
 def dropout_add(x, p, seed, offset=0, residual=None):
@@ -438,6 +475,8 @@ def dropout_add(x, p, seed, offset=0, residual=None):
     drawn again by the backward pass.  offset lets several tensors (or the shards of one) share a seed.  residual: x's shape
     and type, or None.  Differentiable in x and residual."""
     _dropout_checks(x, p, offset, residual)
+    seed, seed_dev = _seed(seed, x.device)
+    _on_gpu(x)
     if _needs_grad(x, residual):
-        return _DropoutAdd.apply(x, residual, p, seed, offset)
-    return _dropout_launch(x, residual, p, seed, offset)
+        return _DropoutAdd.apply(x, residual, p, seed, seed_dev, offset)
+    return _dropout_launch(x, residual, p, seed, seed_dev, offset)

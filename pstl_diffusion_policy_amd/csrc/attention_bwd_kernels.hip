@@ -22,6 +22,11 @@ constexpr int waves_per_simd() {
   return (sizeof(T) == 2 && DK <= 64) || DK <= 32 ? 2 : 1;
 }
 
+template <typename T, int DK>
+constexpr int waves_per_simd_kv() {
+  return sizeof(T) == 2 ? 2 : DK <= 32 ? 2 : 1;
+}
+
 // sum over d of the product of two rows (row fragments; both lane halves)
 template <typename T, int DK>
 __device__ inline float row_dot(const Frag<T> (&x)[DK / 16], const Frag<T> (&y)[DK / 16]) {
@@ -141,24 +146,28 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_q(A
   store_col<T, DK>(row_ptr<T>(a, a.dq, b, hk, r), a.D, hi, acc, live ? a.scale : 0.0f);
 }
 
-// ---- dK, dV: 128 keys per workgroup ------------------------------------------------------------------------------------
+// ---- dK, dV: 64 keys per workgroup --------------------------------------------------------------------------------------
+// Wavefronts 0, 1 take 32 keys each and the even 32-row steps, wavefronts 2, 3 the same keys and the odd steps; their sums are
+// joined in the LDS at the end.  (128 keys per workgroup, all steps in every wavefront: half the workgroups, which a causal mask
+// makes uneven -- 460 us instead of XXX at 4 x 2048 tokens, 16 / 4 heads of 128, bf16.)
 template <typename T, int DK, bool DROP>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_kv(Args a) {
-  constexpr int W = lds_width(DK), BM = block_len<T>(), NS = BM / 32;
+__global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_kv(Args a) {
+  constexpr int W = lds_width(DK), BM = 64;
   typedef Tile<T, W> TL;
-  constexpr int kTileBytes = BM * TL::kRowBytes, kPer = BM * TL::kChunks / 256;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
+  typedef PackedPipe<T, W, BM> Pipe;
+  extern __shared__ __attribute__((aligned(16))) char lds[];      // [2][2][kTileBytes]: Q and dO of two steps
   __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM];
   __shared__ __attribute__((aligned(16))) int row_lim[2][BM];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, col = lane & 31;
-  const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const int unit = work / a.n_tiles, tile = work - unit * a.n_tiles;      // (causal: the first keys are seen by the most rows)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+  const int kg = wave & 1, part = wave >> 1;
+  const Work wk = causal_order((int)blockIdx.x, a.n_tiles, a.B * a.Hk, a.cus_per_xcd);
+  const int unit = wk.unit, key0 = (a.n_tiles - 1 - wk.tile) * 64;      // (causal: the first keys are seen by the most rows)
   const int b = unit / a.Hk, hk = unit - b * a.Hk;
   const Lens n = lens_of(a, b);
-  const int key = tile * 128 + wave * 32 + col;
+  const int key = key0 + kg * 32 + col;
   const bool live = key < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + key] != 0);
-  const int r_end = tile * 128 < n.k ? n.q * a.G : 0;
-  const int r_begin = a.causal ? max(tile * 128 - (n.k - n.q), 0) * a.G / BM * BM : 0;
+  const int r_end = key0 < n.k ? n.q * a.G : 0;
+  const int r_begin = a.causal ? max(key0 - (n.k - n.q), 0) * a.G / BM * BM : 0;
 
   Frag<T> kf[DK / 16], vf[DK / 16];
   load_row_frags<T, DK>(live ? key_ptr<T>(a.k, b, hk, key) : nullptr, live, a.D, hi, kf);
@@ -166,17 +175,15 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_kv(
   f32x16 dk[DK / 32] = {}, dv[DK / 32] = {};
   const uint64_t seed = DROP ? drop_seed(a) : 0;
 
-  u32x4v stage[2][kPer];
-  float st_lse, st_delta;
-  int st_lim;
-  auto fetch = [&](int m0) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int id = tid + 256 * i, row = id / TL::kChunks, d = ((id % TL::kChunks) ^ TL::swz(row)) * TL::kChunkEl, r = m0 + row;
-      const bool ok = r < r_end && d < a.D;
-      stage[0][i] = ok ? *reinterpret_cast<const u32x4v*>(row_ptr<T>(a, a.q, b, hk, r) + d) : u32x4v{0, 0, 0, 0};
-      stage[1][i] = ok ? *reinterpret_cast<const u32x4v*>(row_ptr<T>(a, a.dout, b, hk, r) + d) : u32x4v{0, 0, 0, 0};
-    }
+  const Pipe qp(a, a.q, b, hk, r_end, tid), dop(a, a.dout, b, hk, r_end, tid);
+  auto tile_at = [&](int buf, int which) { return lds + (2 * buf + which) * Pipe::kTileBytes; };
+  if (a.D < W)
+    for (int i = 0; i < 4; ++i) qp.clear(lds + i * Pipe::kTileBytes);
+  float st_lse = 0.0f, st_delta = 0.0f;
+  int st_lim = 0;
+  auto issue = [&](int m0, int buf) {
+    qp.issue(m0, tile_at(buf, 0));
+    dop.issue(m0, tile_at(buf, 1));
     if (tid < BM) {
       const int r = m0 + tid;
       const bool ok = r < r_end;
@@ -185,63 +192,84 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_kv(
       st_lim = ok ? row_limit(a, n, row_query(a, r)) : 0;
     }
   };
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      *reinterpret_cast<u32x4v*>(&lds[buf][0][(tid + 256 * i) * 16]) = stage[0][i];
-      *reinterpret_cast<u32x4v*>(&lds[buf][1][(tid + 256 * i) * 16]) = stage[1][i];
-    }
-    if (tid < BM) row_lse[buf][tid] = st_lse, row_delta[buf][tid] = st_delta, row_lim[buf][tid] = st_lim;
-  };
-  if (r_begin < r_end) {
-    fetch(r_begin);
-    store(0);
-  }
-  __syncthreads();
+  if (r_begin < r_end) issue(r_begin, 0);
   int buf = 0;
   for (int m0 = r_begin; m0 < r_end; m0 += BM, buf ^= 1) {
-    const bool more = m0 + BM < r_end;
-    if (more) fetch(m0 + BM);
-    const char *qt = lds[buf][0], *dot = lds[buf][1];
-    // rows see more keys the later they are: the tile needs no masks when its first row sees the wavefront's last key
-    const bool masked = m0 + BM > r_end || (a.causal && row_lim[buf][0] < tile * 128 + wave * 32 + 32);
+    copies_done();
+    if (m0 + BM > r_end) qp.hide(tile_at(buf, 0), m0), dop.hide(tile_at(buf, 1), m0);
+    if (tid < BM) row_lse[buf][tid] = st_lse, row_delta[buf][tid] = st_delta, row_lim[buf][tid] = st_lim;
+    __syncthreads();
+    if (m0 + BM < r_end) issue(m0 + BM, buf ^ 1);
+    const char *qt = tile_at(buf, 0), *dot = tile_at(buf, 1);
+    const int o0 = 32 * part;
+    f32x16 s = {}, dp = {};
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      f32x16 s = {}, dp = {};
+    for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(qt, o0 + col, t, hi), kf[t], s);
 #pragma unroll
-      for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(qt, 32 * j + col, t, hi), kf[t], s);
+    for (int t = 0; t < DK / 16; ++t) dp = mma(TL::row(dot, o0 + col, t, hi), vf[t], dp);
+    uint32_t w[4];
+    if (DROP) drop_words_keys(seed, (uint32_t)unit, m0 + o0, key, lane, w);
 #pragma unroll
-      for (int t = 0; t < DK / 16; ++t) dp = mma(TL::row(dot, 32 * j + col, t, hi), vf[t], dp);
-      uint32_t w[4];
-      if (DROP) drop_words_keys(seed, (uint32_t)unit, m0 + 32 * j, key, lane, w);
+    for (int q = 0; q < 4; ++q) {
+      const int o = o0 + 8 * q + 4 * hi;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_lse[buf][o]), delta = *reinterpret_cast<const f32x4*>(&row_delta[buf][o]);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int o = 32 * j + 8 * q + 4 * hi;
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_lse[buf][o]), delta = *reinterpret_cast<const f32x4*>(&row_delta[buf][o]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int g = 4 * q + c;
-          const bool see = !masked || key < row_lim[buf][o + c];
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse[c]));
-          const bool keep = !DROP || kept(w, g, a.thr);
-          const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
-          s[g] = see && keep ? p : 0.0f;
-          dp[g] = see ? p * (dpv - delta[c]) : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const Frag<T> p = acc_frag<T>(s, t), ds = acc_frag<T>(dp, t);
-#pragma unroll
-        for (int dt = 0; dt < DK / 32; ++dt) {
-          dv[dt] = mma(TL::col(dot, 32 * j + 16 * t, dt, lane), p, dv[dt]);
-          dk[dt] = mma(TL::col(qt, 32 * j + 16 * t, dt, lane), ds, dk[dt]);
-        }
+      for (int c = 0; c < 4; ++c) {
+        const int g = 4 * q + c;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse[c]));
+        const bool keep = !DROP || kept(w, g, a.thr);
+        const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
+        s[g] = keep ? p : 0.0f;
+        dp[g] = p * (dpv - delta[c]);
       }
     }
-    if (more) store(buf ^ 1);
-    __syncthreads();
+    // rows see more keys the later they are: no masks when the step's first row sees the wavefront's last key
+    if (m0 + BM > r_end || (a.causal && row_lim[buf][o0] < key0 + kg * 32 + 32)) {
+      asm volatile("");
+#pragma unroll
+      for (int g = 0; g < 16; ++g) {
+        const bool see = key < row_lim[buf][o0 + 8 * (g >> 2) + 4 * hi + (g & 3)];
+        s[g] = see ? s[g] : 0.0f, dp[g] = see ? dp[g] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Frag<T> p = acc_frag<T>(s, t), ds = acc_frag<T>(dp, t);
+#pragma unroll
+      for (int dt = 0; dt < DK / 32; ++dt) {
+        dv[dt] = mma(TL::col(dot, o0 + 16 * t, dt, lane), p, dv[dt]);
+        dk[dt] = mma(TL::col(qt, o0 + 16 * t, dt, lane), ds, dk[dt]);
+      }
+    }
   }
+  // the odd steps' sums into the even steps' wavefronts: (register, lane) by (register, lane)
+  __syncthreads();
+  float* x = reinterpret_cast<float*>(lds) + kg * (DK / 32) * 2048 + lane * 4;
+  auto give = [&](const f32x16 (&v)[DK / 32]) {
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(x + dt * 1024 + q * 256) = f32x4{v[dt][4 * q], v[dt][4 * q + 1], v[dt][4 * q + 2], v[dt][4 * q + 3]};
+  };
+  auto take = [&](f32x16 (&v)[DK / 32]) {
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(x + dt * 1024 + q * 256);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[dt][4 * q + c] += y[c];
+      }
+  };
+  if (part) give(dk);
+  __syncthreads();
+  if (!part) take(dk);
+  __syncthreads();
+  if (part) give(dv);
+  __syncthreads();
+  if (part) return;
+  take(dv);
   if (key >= a.Lk) return;
   if (!live) {      // (a hidden key's column holds sums of no meaning, infinities among them: it is written as zeros)
 #pragma unroll
@@ -361,6 +389,7 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(4))) void k_attn_bwd_short
 template <typename T, int DK, bool DROP>
 int launch(const Args& a0, hipStream_t st) {
   Args a = a0;
+  a.cus_per_xcd = device_cus() >= 8 ? device_cus() / 8 : 1;
   const int64_t units = (int64_t)a.B * a.Hk;
   if (a.Lk <= 32) {
     constexpr int NW = short_waves<T, DK>(4);
@@ -379,9 +408,11 @@ int launch(const Args& a0, hipStream_t st) {
     hipLaunchKernelGGL((k_attn_bwd_q<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), 0, st, a);
     if (int e = launch_status()) return e;
   }
-  a.n_tiles = ceil_div(a.Lk, 128);
+  a.n_tiles = ceil_div(a.Lk, 64);
   if (units * a.n_tiles >= (1ll << 31)) return PSTL_ERR_SHAPE;
-  hipLaunchKernelGGL((k_attn_bwd_kv<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), 0, st, a);
+  constexpr int kBytes = 4 * 64 * lds_width(DK) * (int)sizeof(T) > 2 * 32 * DK * 4 ? 4 * 64 * lds_width(DK) * (int)sizeof(T) : 2 * 32 * DK * 4;
+  if (int e = allow_lds<k_attn_bwd_kv<T, DK, DROP>>(kBytes)) return e;
+  hipLaunchKernelGGL((k_attn_bwd_kv<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), kBytes, st, a);
   return launch_status();
 }
 template <typename T, int DK>

@@ -19,129 +19,139 @@ constexpr int block_keys() {
 }
 
 // ---- many rows: 128 packed rows per workgroup, 32 per wavefront; tiles of keys and values shared through the LDS -----------
+// The scores of the NEXT 32 keys are formed (matrix pipe) beside the exponentials of the present ones (vector pipe).  16-bit types:
+// fragments of keys are read from the LDS a step before their product, so that a tile of keys is used up one tile ahead of its
+// values.
+// The maximum that the exponents are taken against moves only when a score exceeds it by more than 2^8: P is then at most 256
+// in 32 bits, the sums stay exact to their rounding, and the accumulators are hardly ever rescaled.
 template <typename T, int DK, bool DROP>
-__global__ __launch_bounds__(256, 2) void k_attn_fwd(Args a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DK > 64 ? 1 : 2) void k_attn_fwd(Args a) {
   constexpr int W = lds_width(DK), BN = block_keys<T>(), NS = BN / 32;
+  typedef RowPipe<T, W, BN> Pipe;
   typedef Tile<T, W> TL;
-  constexpr int kTileBytes = BN * TL::kRowBytes, kPer = BN * TL::kChunks / 256;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, col = lane & 31;
-  const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const int unit = work / a.n_tiles, tile = a.n_tiles - 1 - (work - unit * a.n_tiles);   // (causal: the longest first)
+  __shared__ __attribute__((aligned(16))) char lds_k[2][Pipe::kTileBytes], lds_v[2][Pipe::kTileBytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+  const Work wk = causal_order((int)blockIdx.x, a.n_tiles, a.B * a.Hk, a.cus_per_xcd);
+  const int unit = wk.unit, base = wk.tile * 128;
   const int b = unit / a.Hk, hk = unit - b * a.Hk;
   const Lens n = lens_of(a, b);
-  const int r0 = tile * 128 + wave * 32, r = r0 + col;
-  const int qi = row_query(a, r);
+  const int r0 = base + wave * 32, r = r0 + col, qi = row_query(a, r);
   const bool live = r < a.R && qi < n.q;
   const int lim = live ? row_limit(a, n, qi) : 0;
+  Frag<T> qf[DK / 16];
+  load_row_frags<T, DK>(live ? row_ptr<T>(a, a.q, b, hk, r) : nullptr, live, a.D, hi, qf);
   // keys that some row of the workgroup sees; keys that every live row of the wavefront sees
-  const int q_first = row_query(a, tile * 128), q_last = min(row_query(a, min(tile * 128 + 127, a.R - 1)), n.q - 1);
+  const int q_first = row_query(a, base), q_last = min(row_query(a, min(base + 127, a.R - 1)), n.q - 1);
   const int kend = q_first < n.q ? row_limit(a, n, q_last) : 0;
   const int q_wave = row_query(a, r0), all_see = a.causal ? max(min(q_wave + n.k - n.q + 1, n.k), 0) : n.k;
 
-  Frag<T> qf[DK / 16];
-  load_row_frags<T, DK>(live ? row_ptr<T>(a, a.q, b, hk, r) : nullptr, live, a.D, hi, qf);
   f32x16 acc[DK / 32] = {};
   float m = -INFINITY, l = 0.0f;
   const uint64_t seed = DROP ? drop_seed(a) : 0;
 
-  u32x4v stage[2][kPer];
-  auto fetch = [&](int k0) {
+  const Pipe kp(key_ptr<T>(a.k, b, hk, 0), a.k.sl, a.Lk, a.D, tid), vp(key_ptr<T>(a.v, b, hk, 0), a.v.sl, a.Lk, a.D, tid);
+  KeyMask<BN> km(a, b, n.k, lane);
+  if (a.D < W) kp.clear(lds_k[0]), kp.clear(lds_k[1]), vp.clear(lds_v[0]), vp.clear(lds_v[1]);
+  constexpr bool kAhead = NS == 2 && !(DROP && DK == 128);      // (the draws need the registers there)
+  Frag<T> kf[kAhead ? DK / 16 : 1];      // the fragments of the next scores
+  auto read_keys = [&](const char* kt, int j) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int id = tid + 256 * i, row = id / TL::kChunks, c = (id % TL::kChunks) ^ TL::swz(row), key = k0 + row;
-      const int d = c * TL::kChunkEl;
-      bool ok = key < n.k && d < a.D;
-      if (ok && a.key_mask) ok = a.key_mask[b * a.mask_sb + key] != 0;   // hidden keys may hold anything: 0 * NaN is NaN
-      stage[0][i] = ok ? *reinterpret_cast<const u32x4v*>(key_ptr<T>(a.k, b, hk, key) + d) : u32x4v{0, 0, 0, 0};
-      stage[1][i] = ok ? *reinterpret_cast<const u32x4v*>(key_ptr<T>(a.v, b, hk, key) + d) : u32x4v{0, 0, 0, 0};
-    }
+    for (int t = 0; t < (kAhead ? DK / 16 : 0); ++t) kf[t] = TL::row(kt, 32 * j + col, t, hi);
   };
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      *reinterpret_cast<u32x4v*>(&lds[buf][0][(tid + 256 * i) * 16]) = stage[0][i];
-      *reinterpret_cast<u32x4v*>(&lds[buf][1][(tid + 256 * i) * 16]) = stage[1][i];
-    }
-  };
+  f32x16 s = {};
   if (kend > 0) {
-    fetch(0);
-    store(0);
+    kp.issue(0, lds_k[0]);
+    copies_done();
+    __syncthreads();
+    vp.issue(0, lds_v[0]);
+    km.fetch(0);
+    if (BN < kend) kp.issue(BN, lds_k[1]);
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(lds_k[0], col, t, hi), qf[t], s);
+    read_keys(lds_k[0], 1);
   }
-  __syncthreads();
   int buf = 0;
   for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
-    const bool more = k0 + BN < kend;
-    if (more) fetch(k0 + BN);
-    const char *kt = lds[buf][0], *vt = lds[buf][1];
-    f32x16 s[NS] = {};
-#pragma unroll
-    for (int j = 0; j < NS; ++j)
-#pragma unroll
-      for (int t = 0; t < DK / 16; ++t) s[j] = mma(TL::row(kt, 32 * j + col, t, hi), qf[t], s[j]);
-    if (k0 + BN > all_see || a.key_mask) {
-      uint64_t vis = ~0ull;
-      if (a.key_mask) {
-        const int key = k0 + lane;
-        vis = __ballot(key < n.k && lane < BN && a.key_mask[b * a.mask_sb + key] != 0) >> (4 * hi);
-      }
-#pragma unroll
-      for (int j = 0; j < NS; ++j)
-#pragma unroll
-        for (int g = 0; g < 16; ++g) {
-          const int o = 32 * j + 8 * (g >> 2) + (g & 3);
-          const bool see = k0 + o + 4 * hi < lim && ((vis >> o) & 1);
-          s[j][g] = see ? s[j][g] : -INFINITY;
-        }
+    copies_done();         // V of this tile, K of the next
+    const uint64_t visible = km.bits(k0);
+    if (k0 + BN > n.k || a.key_mask) vp.hide(lds_v[buf], visible);
+    __syncthreads();
+    if (k0 + BN < kend) vp.issue(k0 + BN, lds_v[buf ^ 1]), km.fetch(k0 + BN);
+    // (without kAhead the second half of this tile's keys is still to be read: their buffer is filled again behind that)
+    if (kAhead || NS == 1) {
+      if (k0 + 2 * BN < kend) kp.issue(k0 + 2 * BN, lds_k[buf]);
     }
-    float mx = s[0][0];
+    const char *vt = lds_v[buf], *kt = lds_k[buf ^ 1];
 #pragma unroll
-    for (int j = 0; j < NS; ++j)
+    for (int j = 0; j < NS; ++j) {
+      Frag<T> vf[DK / 32];      // the first half of the values' fragments (both do not fit the registers at DK = 128)
+      if (kAhead) {
 #pragma unroll
-      for (int g = 0; g < 16; ++g) mx = fmaxf(mx, s[j][g]);
-    const float m_new = fmaxf(m, half_max(mx) * a.c), mu = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m - mu);
-    m = m_new;
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NS; ++j)
-#pragma unroll
-      for (int g = 0; g < 16; ++g) {
-        s[j][g] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][g], a.c, -mu));
-        sum += s[j][g];
+        for (int dt = 0; dt < DK / 32; ++dt) vf[dt] = TL::col(vt, 32 * j, dt, lane);
       }
-    l = __builtin_fmaf(l, alpha, sum);
-    if (DROP) {
+      if (k0 + BN > all_see || a.key_mask) {
+        asm volatile("");      // (a branch, not a select per score)
+        const uint32_t see = seen_bits<false>((uint32_t)(visible >> (32 * j)), min(max(lim - k0 - 32 * j, 0), 32), lane) >> (4 * hi);
 #pragma unroll
-      for (int j = 0; j < NS; ++j) {
+        for (int x = 0; x < 16; ++x) s[x] = (see >> (8 * (x >> 2) + (x & 3))) & 1 ? s[x] : -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int x = 1; x < 16; ++x) mx = fmaxf(mx, s[x]);
+      mx *= a.c;
+      if (__any(mx > m + 8.0f)) {
+        const float to = fmaxf(m, half_max(mx)), alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
+        m = to;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DK / 32; ++dt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) acc[dt][x] *= alpha;
+      }
+      // (behind the last tile: scores of whatever the buffer holds, never looked at)
+      f32x16 next = {};
+#pragma unroll
+      for (int t = 0; t < DK / 16; ++t) {
+        if constexpr (kAhead)
+          next = mma(kf[t], qf[t], next);
+        else
+          next = mma(j + 1 < NS ? TL::row(lds_k[buf], 32 * (j + 1) + col, t, hi) : TL::row(kt, col, t, hi), qf[t], next);
+      }
+      read_keys(kt, j);
+      const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.c, -mu));
+        l += s[x];
+      }
+      if (DROP) {
         uint32_t w[4];
         drop_words_rows(seed, (uint32_t)unit, r, k0 + 32 * j, lane, w);
 #pragma unroll
-        for (int g = 0; g < 16; ++g) s[j][g] = kept(w, g, a.thr) ? s[j][g] : 0.0f;
+        for (int x = 0; x < 16; ++x) s[x] = kept(w, x, a.thr) ? s[x] : 0.0f;
       }
-    }
-    if (__any(alpha != 1.0f)) {
-#pragma unroll
-      for (int dt = 0; dt < DK / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 16; ++g) acc[dt][g] *= alpha;
-    }
-#pragma unroll
-    for (int j = 0; j < NS; ++j)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const Frag<T> p = acc_frag<T>(s[j], t);
+        const Frag<T> p = acc_frag<T>(s, t);
 #pragma unroll
-        for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = mma(TL::col(vt, 32 * j + 16 * t, dt, lane), p, acc[dt]);
+        for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = mma(kAhead && t == 0 ? vf[dt] : TL::col(vt, 32 * j + 16 * t, dt, lane), p, acc[dt]);
       }
-    if (more) store(buf ^ 1);
-    __syncthreads();
+      s = next;
+      if (!kAhead && NS == 2 && j == 0) {
+        __syncthreads();
+        if (k0 + 2 * BN < kend) kp.issue(k0 + 2 * BN, lds_k[buf]);
+      }
+    }
   }
   l = half_sum(l);
   if (r >= a.R) return;
-  const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : (l == 0.0f ? 0.0f : l);   // (a NaN sum stays one)
+  const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : l;      // (0 for a row that sees nothing; a NaN sum stays one)
   if (hi == 0 && a.lse) a.lse[(int64_t)unit * a.R + r] = live && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
-  store_col<T, DK>(row_ptr<T>(a, a.o, b, hk, r), a.D, hi, acc, live ? inv : 0.0f);
+  if (!live) {
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = f32x16{};
+  }
+  store_col<T, DK>(row_ptr<T>(a, a.o, b, hk, r), a.D, hi, acc, inv);
 }
 
 // ---- at most 32 keys: one wavefront per 32 packed rows, or per pair of units of at most 16 rows and keys -----------------
@@ -407,7 +417,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Args a, float gain) {
 template <typename T, int DK, bool DROP>
 int launch(const Args& a0, const FwdPlan& p, hipStream_t st) {
   Args a = a0;
-  a.n_tiles = p.n_tiles, a.splits = p.splits, a.tiles_per_split = p.tiles_per_split;
+  a.n_tiles = p.n_tiles, a.splits = p.splits, a.tiles_per_split = p.tiles_per_split, a.cus_per_xcd = p.cus_per_xcd;
   const int64_t units = (int64_t)a.B * a.Hk;
   if (p.kind == kManyRows) {
     hipLaunchKernelGGL((k_attn_fwd<T, DK, DROP>), dim3((unsigned)(units * p.n_tiles)), dim3(256), 0, st, a);
@@ -422,14 +432,7 @@ int launch(const Args& a0, const FwdPlan& p, hipStream_t st) {
       hipLaunchKernelGGL((k_attn_fwd_short<T, DK, DROP, false>), grid, block, 0, st, a);
   } else {
     constexpr int kTile2 = 2 * 32 * lds_width(DK) * (int)sizeof(T), kJoin = 32 * DK * 4, kBytes = 4 * (kTile2 > kJoin ? kTile2 : kJoin);
-    static DeviceOnce once;
-    const int dev = current_device();
-    if (!once.done(dev)) {
-      if (hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_fwd_few<T, DK, DROP>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              kBytes) != hipSuccess)
-        return PSTL_ERR_LAUNCH;
-      once.set(dev);
-    }
+    if (int e = allow_lds<k_attn_fwd_few<T, DK, DROP>>(kBytes)) return e;
     hipLaunchKernelGGL((k_attn_fwd_few<T, DK, DROP>), dim3((unsigned)(units * p.n_tiles * p.splits)), dim3(256), kBytes, st, a);
     if (p.splits > 1) {
       if (int e = launch_status()) return e;

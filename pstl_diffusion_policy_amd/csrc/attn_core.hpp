@@ -234,7 +234,7 @@ struct Args {
   float scale, c;             // c = scale log2(e)
   uint32_t thr;               // a probability is dropped when its byte is below thr
   float keep_inv;             // 256 / (256 - thr)
-  int n_tiles, splits, tiles_per_split;
+  int n_tiles, splits, tiles_per_split, cus_per_xcd;
 };
 
 __device__ inline int row_query(const Args& a, int r) { return a.G == 1 ? r : (int)__umulhi((uint32_t)r, a.g_magic); }
@@ -272,6 +272,155 @@ __device__ inline int xcd_order(int x, int n) {
   const int q = n >> 3, rem = n & 7, xcd = x & 7;
   return xcd * q + min(xcd, rem) + (x >> 3);
 }
+
+// Order of the workgroups of a causal launch.  All tiles of a unit stay on one XCD (or on 8 / units of them); inside an XCD the
+// longest come first, and every second round of one tile per compute unit runs backwards, so that the two workgroups a compute
+// unit holds at once are a long and a short one.  Where the units do not divide the XCDs evenly: xcd_order, longest first.
+struct Work {
+  int unit, tile;
+};
+__device__ inline Work causal_order(int x, int n_tiles, int units, int cus_per_xcd) {
+  const int total = n_tiles * units, xcd = x & 7, q = x >> 3;
+  int share = 0;                      // XCDs that share a unit's tiles
+  if (units % 8 == 0) share = 1;
+  else if (8 % units == 0 && n_tiles % (8 / units) == 0) share = 8 / units;
+  if (share == 0) {
+    const int w = xcd_order(x, total), unit = w / n_tiles;
+    return Work{unit, n_tiles - 1 - (w - unit * n_tiles)};
+  }
+  const int per = total >> 3, round = q / cus_per_xcd, i = q - round * cus_per_xcd, width = min(cus_per_xcd, per - round * cus_per_xcd);
+  const int pos = round * cus_per_xcd + ((round & 1) ? width - 1 - i : i);
+  const int here = share > 1 ? 1 : units >> 3, u = pos % here;      // units of this XCD
+  return share > 1 ? Work{xcd / share, n_tiles - 1 - (pos * share + xcd % share)} : Work{xcd * here + u, n_tiles - 1 - pos / here};
+}
+
+// ---- tiles of keys and values, copied to the LDS without passing through registers ----------------------------------------
+// 256 threads copy BN rows with global_load_lds_dwordx4: lane l of a wavefront writes 16 bytes at the wavefront's LDS address +
+// 16 l, so the swizzle is a permutation of the chunks that the lanes fetch.  The copies are inline asm because the compiler would
+// wait for them before any LDS read; copies_done() is the wait.  Rows past the tensor repeat its last row; rows that the mask or
+// the lengths hide are overwritten by zeros after their arrival where a product contracts over them (a hidden NaN times a zero
+// probability is NaN).
+__device__ inline void copy16(const void* g, uint32_t lds_wave) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_wave) : "memory", "m0");
+}
+__device__ inline void copy16(const void* base, uint32_t offset, uint32_t lds_wave) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds_wave) : "memory", "m0");
+}
+__device__ inline void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ inline uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+template <typename T>
+__device__ inline T* uniform_ptr(T* p) {      // (readfirstlane gives a SIGNED word: each half through an unsigned one)
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return reinterpret_cast<T*>(((uint64_t)hi << 32) | lo);
+}
+
+template <typename T, int W, int BN>
+struct RowPipe {      // one tensor's rows (keys) of one unit
+  typedef Tile<T, W> TL;
+  static constexpr int kTileBytes = BN * TL::kRowBytes, kPer = BN * TL::kChunks / 256, kRowStep = 256 / TL::kChunks;
+  const char* base;
+  int64_t stride;      // bytes
+  int rows, D, tid;    // rows of the tensor
+  bool near;           // a tile's rows lie within 2^31 bytes
+  __device__ RowPipe(const T* first, int64_t stride_el, int rows_, int D_, int tid_)
+      : base(uniform_ptr(reinterpret_cast<const char*>(first))), stride(stride_el * (int)sizeof(T)), rows(rows_), D(D_), tid(tid_) {
+    near = stride >= 0 && stride < (1ll << 31) / BN;
+  }
+  __device__ inline int row(int i) const { return tid / TL::kChunks + i * kRowStep; }
+  __device__ inline int chunk(int i) const { return (tid % TL::kChunks) ^ TL::swz(row(i)); }
+  // chunks past D never arrive: they are zeroed once
+  __device__ inline void clear(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (chunk(i) * TL::kChunkEl >= D) *reinterpret_cast<u32x4v*>(tile + (tid + 256 * i) * 16) = u32x4v{0, 0, 0, 0};
+  }
+  __device__ inline void issue(int k0, const char* tile) const {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile) + (tid >> 6) * 1024);
+    if (near && k0 + BN <= rows) {
+      const char* at = base + k0 * stride;
+      const uint32_t off = (uint32_t)(tid / TL::kChunks) * (uint32_t)stride;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (chunk(i) * TL::kChunkEl < D) copy16(at + i * kRowStep * stride, off + chunk(i) * 16, to + i * 4096);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (chunk(i) * TL::kChunkEl < D) copy16(base + min(k0 + row(i), rows - 1) * stride + chunk(i) * 16, to + i * 4096);
+    }
+  }
+  __device__ inline void hide(char* tile, uint64_t visible) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (!((visible >> row(i)) & 1)) *reinterpret_cast<u32x4v*>(tile + (tid + 256 * i) * 16) = u32x4v{0, 0, 0, 0};
+  }
+};
+template <typename T, int W, int BM>
+struct PackedPipe {      // one tensor's packed rows [0, end) of one unit
+  typedef Tile<T, W> TL;
+  static constexpr int kTileBytes = BM * TL::kRowBytes, kPer = BM * TL::kChunks / 256, kRowStep = 256 / TL::kChunks;
+  const Args& a;
+  const char* base;
+  int64_t sl, sh;      // bytes
+  int end, tid;
+  uint32_t off;        // of this thread's first row in a tile
+  bool near;           // a tile is a fixed pattern within 2^31 bytes
+  __device__ PackedPipe(const Args& a_, const Mat& m, int b, int hk, int end_, int tid_) : a(a_), end(end_), tid(tid_) {
+    base = uniform_ptr(m.p + (b * m.sb + (int64_t)(hk * a.G) * m.sh) * (int)sizeof(T));
+    sl = m.sl * (int)sizeof(T), sh = m.sh * (int)sizeof(T);
+    near = kRowStep % a.G == 0 && sl >= 0 && sh >= 0 && sl < (1ll << 30) / BM && sh < (1ll << 30) / BM;
+    const int i = row_query(a, tid / TL::kChunks), g = tid / TL::kChunks - i * a.G;
+    off = near ? (uint32_t)i * (uint32_t)sl + (uint32_t)g * (uint32_t)sh : 0;
+  }
+  __device__ inline int row(int i) const { return tid / TL::kChunks + i * kRowStep; }
+  __device__ inline int chunk(int i) const { return (tid % TL::kChunks) ^ TL::swz(row(i)); }
+  __device__ inline void clear(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (chunk(i) * TL::kChunkEl >= a.D) *reinterpret_cast<u32x4v*>(tile + (tid + 256 * i) * 16) = u32x4v{0, 0, 0, 0};
+  }
+  __device__ inline void issue(int m0, const char* tile) const {      // m0: a multiple of BM
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile) + (tid >> 6) * 1024);
+    if (near && m0 + BM <= end) {
+      const char* at = base + row_query(a, m0) * sl;
+      const int64_t step = (uint32_t)row_query(a, kRowStep) * sl;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (chunk(i) * TL::kChunkEl < a.D) copy16(at + i * step, off + chunk(i) * 16, to + i * 4096);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (chunk(i) * TL::kChunkEl < a.D) {
+          const int r = min(m0 + row(i), end - 1), q = row_query(a, r);
+          copy16(base + q * sl + (r - q * a.G) * sh + chunk(i) * 16, to + i * 4096);
+        }
+    }
+  }
+  __device__ inline void hide(char* tile, int m0) const {      // rows past the end: zeros
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (m0 + row(i) >= end) *reinterpret_cast<u32x4v*>(tile + (tid + 256 * i) * 16) = u32x4v{0, 0, 0, 0};
+  }
+};
+// which keys of a tile are visible to anyone, as bits; the mask's bytes are fetched a tile ahead
+template <int BN>
+struct KeyMask {
+  const uint8_t* mask;
+  int n_k, last, lane;
+  uint8_t next;
+  __device__ KeyMask(const Args& a, int b, int n_k_, int lane_)
+      : mask(a.key_mask ? a.key_mask + b * a.mask_sb : nullptr), n_k(n_k_), last(a.Lk - 1), lane(lane_), next(1) {}
+  __device__ inline void fetch(int k0) {
+    if (mask) next = mask[min(k0 + lane, last)];
+  }
+  __device__ inline uint64_t bits(int k0) const {
+    const uint64_t all = BN == 64 ? ~0ull : (1ull << BN) - 1;
+    if (mask) return __ballot(lane < BN && k0 + lane < n_k && next != 0);
+    return k0 + BN > n_k ? (n_k > k0 ? (1ull << (n_k - k0)) - 1 : 0) : all;
+  }
+};
 
 // row fragments of one packed row straight from global memory; zeros past D and for rows that are not there
 template <typename T, int DK>

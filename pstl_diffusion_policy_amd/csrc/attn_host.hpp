@@ -51,12 +51,24 @@ inline int attn_args(const pstl_attn* c, Args* a, Check what) {
   return PSTL_OK;
 }
 
+// lets a kernel use `bytes` of dynamic LDS (more than 64 KB must be asked for), once per device
+template <auto Kernel>
+inline int allow_lds(int bytes) {
+  static DeviceOnce once;
+  const int dev = current_device();
+  if (once.done(dev)) return PSTL_OK;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return PSTL_ERR_LAUNCH;
+  once.set(dev);
+  return PSTL_OK;
+}
+
 // ---- forward ---------------------------------------------------------------------------------------------------------
 constexpr int kMaxSplits = 1024;
 enum Kind { kManyRows, kShort, kShortPairs, kFewRows };
 struct FwdPlan {
   Kind kind;
-  int n_tiles, splits, tiles_per_split;
+  int n_tiles, splits, tiles_per_split, cus_per_xcd;
 };
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -66,7 +78,7 @@ inline bool in_pairs(const Args& a) {
 }
 inline FwdPlan plan_forward(const Args& a, int cus) {
   const int64_t units = (int64_t)a.B * a.Hk;
-  FwdPlan p = {kManyRows, ceil_div(a.R, 128), 1, 0};
+  FwdPlan p = {kManyRows, ceil_div(a.R, 128), 1, 0, cus >= 8 ? cus / 8 : 1};
   if (a.Lk <= 32) {
     p.kind = in_pairs(a) ? kShortPairs : kShort;
     p.n_tiles = ceil_div(a.R, 32);

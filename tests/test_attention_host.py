@@ -32,6 +32,17 @@ def test_structures_match_the_header():
                 want.append(ctypes.c_void_p if "*" in var else {"int32_t": ctypes.c_int32, "float": ctypes.c_float,
                             "uint64_t": ctypes.c_uint64, "int64_t": ctypes.c_int64, "pstl_attn_mat": ffi.AttnMat}[ctype])
         assert [(n, t) for n, t in cls._fields_] == list(zip(fields, want)), name
+    from pstl_diffusion_policy_amd import attention as A
+    for packed, cls in ((A._ATTN, ffi.Attn), (A._ROPE, ffi.QkRope)):      # the bytes attention.py hands over
+        flat = [t for f in cls._fields_ for t in (f[1]._fields_ if f[1] is ffi.AttnMat else [f])]
+        assert packed.size == ctypes.sizeof(cls) and len(packed.unpack(bytes(packed.size))) == len(flat)
+        values = list(range(1, len(flat) + 1))
+        a = cls.from_buffer_copy(packed.pack(*values))
+        got = []
+        for n, t in cls._fields_:
+            x = getattr(a, n)
+            got += [getattr(x, m) for m, _ in x._fields_] if t is ffi.AttnMat else [x]
+        assert got == values
 
 
 @pytest.mark.parametrize("change, error, text", [
@@ -104,6 +115,7 @@ def test_scale_seed_and_layout_checks():
     (dict(inv_freq=torch.ones(16)), TypeError, "float64"),
     (dict(inv_freq=torch.ones(4, dtype=torch.float64)), ValueError, "multiple of 16"),
     (dict(inv_freq=torch.ones(24, dtype=torch.float64)), ValueError, "multiple of 16"),
+    (dict(eps=-1.0), ValueError, "eps"),
     (dict(), RuntimeError, "on the GPU"),
 ])
 def test_qk_norm_rope_refuses(change, error, text):

@@ -18,13 +18,12 @@ constexpr int block_len() {
   return sizeof(T) == 2 ? 64 : 32;
 }
 template <typename T, int DK>
-constexpr int waves_per_simd() {
-  return (sizeof(T) == 2 && DK <= 64) || DK <= 32 ? 2 : 1;
+constexpr int waves_per_simd_q() {
+  return sizeof(T) == 2 ? 2 : DK <= 32 ? 2 : 1;
 }
-
 template <typename T, int DK>
 constexpr int waves_per_simd_kv() {
-  return sizeof(T) == 2 ? 2 : DK <= 32 ? 2 : 1;
+  return sizeof(T) == 2 && DK <= 64 ? 2 : DK <= 32 ? 2 : 1;
 }
 
 // sum over d of the product of two rows (row fragments; both lane halves)
@@ -38,27 +37,31 @@ __device__ inline float row_dot(const Frag<T> (&x)[DK / 16], const Frag<T> (&y)[
   return half_sum(s);
 }
 
-// ---- dQ: 128 packed rows per workgroup -------------------------------------------------------------------------------
+// ---- dQ: 128 packed rows per workgroup, 32 per wavefront ---------------------------------------------------------------
 template <typename T, int DK, bool DROP>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_q(Args a) {
+__global__ __launch_bounds__(256, (waves_per_simd_q<T, DK>())) void k_attn_bwd_q(Args a) {
   constexpr int W = lds_width(DK), BN = block_len<T>(), NS = BN / 32;
   typedef Tile<T, W> TL;
-  constexpr int kTileBytes = BN * TL::kRowBytes, kPer = BN * TL::kChunks / 256;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, col = lane & 31;
-  const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const int unit = work / a.n_tiles, tile = a.n_tiles - 1 - (work - unit * a.n_tiles);
+  typedef RowPipe<T, W, BN> Pipe;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][Pipe::kTileBytes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+  const Work wk = causal_order((int)blockIdx.x, a.n_tiles, a.B * a.Hk, a.cus_per_xcd);
+  const int unit = wk.unit, base = wk.tile * 128;
   const int b = unit / a.Hk, hk = unit - b * a.Hk;
   const Lens n = lens_of(a, b);
-  const int r0 = tile * 128 + wave * 32, r = r0 + col;
+  const int r0 = base + wave * 32, r = r0 + col;
   const int qi = row_query(a, r);
   const bool live = r < a.R && qi < n.q;
   const int lim = live ? row_limit(a, n, qi) : 0;
-  const int q_first = row_query(a, tile * 128), q_last = min(row_query(a, min(tile * 128 + 127, a.R - 1)), n.q - 1);
+  const int q_first = row_query(a, base), q_last = min(row_query(a, min(base + 127, a.R - 1)), n.q - 1);
   const int kend = q_first < n.q ? row_limit(a, n, q_last) : 0;
   const int q_wave = row_query(a, r0);
   const int all_see = r0 + 32 > a.R || row_query(a, r0 + 31) >= n.q ? 0 : a.causal ? max(min(q_wave + n.k - n.q + 1, n.k), 0) : n.k;
 
+  const Pipe kp(key_ptr<T>(a.k, b, hk, 0), a.k.sl, a.Lk, a.D, tid), vp(key_ptr<T>(a.v, b, hk, 0), a.v.sl, a.Lk, a.D, tid);
+  KeyMask<BN> km(a, b, n.k, lane);
+  if (a.D < W) kp.clear(lds[0][0]), kp.clear(lds[1][0]), vp.clear(lds[0][1]), vp.clear(lds[1][1]);
+  if (kend > 0) km.fetch(0), kp.issue(0, lds[0][0]), vp.issue(0, lds[0][1]);
   Frag<T> qf[DK / 16], dof[DK / 16];
   load_row_frags<T, DK>(live ? row_ptr<T>(a, a.q, b, hk, r) : nullptr, live, a.D, hi, qf);
   load_row_frags<T, DK>(live ? row_ptr<T>(a, a.dout, b, hk, r) : nullptr, live, a.D, hi, dof);
@@ -72,42 +75,15 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_q(A
   }
   f32x16 acc[DK / 32] = {};
   const uint64_t seed = DROP ? drop_seed(a) : 0;
-
-  u32x4v stage[2][kPer];
-  auto fetch = [&](int k0) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int id = tid + 256 * i, row = id / TL::kChunks, c = (id % TL::kChunks) ^ TL::swz(row), key = k0 + row;
-      const int d = c * TL::kChunkEl;
-      bool ok = key < n.k && d < a.D;
-      if (ok && a.key_mask) ok = a.key_mask[b * a.mask_sb + key] != 0;
-      stage[0][i] = ok ? *reinterpret_cast<const u32x4v*>(key_ptr<T>(a.k, b, hk, key) + d) : u32x4v{0, 0, 0, 0};
-      stage[1][i] = ok ? *reinterpret_cast<const u32x4v*>(key_ptr<T>(a.v, b, hk, key) + d) : u32x4v{0, 0, 0, 0};
-    }
-  };
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      *reinterpret_cast<u32x4v*>(&lds[buf][0][(tid + 256 * i) * 16]) = stage[0][i];
-      *reinterpret_cast<u32x4v*>(&lds[buf][1][(tid + 256 * i) * 16]) = stage[1][i];
-    }
-  };
-  if (kend > 0) {
-    fetch(0);
-    store(0);
-  }
-  __syncthreads();
   int buf = 0;
   for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
-    const bool more = k0 + BN < kend;
-    if (more) fetch(k0 + BN);
+    copies_done();
+    const uint64_t visible = km.bits(k0);
+    if (k0 + BN > n.k || a.key_mask) kp.hide(lds[buf][0], visible);      // (dP of a hidden key is selected away)
+    __syncthreads();
+    if (k0 + BN < kend) km.fetch(k0 + BN), kp.issue(k0 + BN, lds[buf ^ 1][0]), vp.issue(k0 + BN, lds[buf ^ 1][1]);
     const char *kt = lds[buf][0], *vt = lds[buf][1];
     const bool masked = k0 + BN > all_see || a.key_mask;
-    uint64_t vis = ~0ull;
-    if (a.key_mask) {
-      const int key = k0 + lane;
-      vis = __ballot(key < n.k && lane < BN && a.key_mask[b * a.mask_sb + key] != 0) >> (4 * hi);
-    }
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       f32x16 s = {}, dp = {};
@@ -125,12 +101,10 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_q(A
         s[g] = p * (dpv - delta);
       }
       if (masked) {
+        asm volatile("");      // (a branch, not a select per score)
+        const uint32_t see = seen_bits<false>((uint32_t)(visible >> (32 * j)), min(max(lim - k0 - 32 * j, 0), 32), lane) >> (4 * hi);
 #pragma unroll
-        for (int g = 0; g < 16; ++g) {
-          const int o = 32 * j + 8 * (g >> 2) + (g & 3);
-          const bool see = k0 + o + 4 * hi < lim && ((vis >> o) & 1);
-          s[g] = see ? s[g] : 0.0f;
-        }
+        for (int g = 0; g < 16; ++g) s[g] = (see >> (8 * (g >> 2) + (g & 3))) & 1 ? s[g] : 0.0f;
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -139,25 +113,41 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DK>())) void k_attn_bwd_q(A
         for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = mma(TL::col(kt, 32 * j + 16 * t, dt, lane), ds, acc[dt]);
       }
     }
-    if (more) store(buf ^ 1);
-    __syncthreads();
   }
   if (r >= a.R) return;
-  store_col<T, DK>(row_ptr<T>(a, a.dq, b, hk, r), a.D, hi, acc, live ? a.scale : 0.0f);
+  if (!live) {
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = f32x16{};
+  }
+  store_col<T, DK>(row_ptr<T>(a, a.dq, b, hk, r), a.D, hi, acc, a.scale);
 }
 
 // ---- dK, dV: 64 keys per workgroup --------------------------------------------------------------------------------------
 // Wavefronts 0, 1 take 32 keys each and the even 32-row steps, wavefronts 2, 3 the same keys and the odd steps; their sums are
 // joined in the LDS at the end.  (128 keys per workgroup, all steps in every wavefront: half the workgroups, which a causal mask
-// makes uneven -- 460 us instead of XXX at 4 x 2048 tokens, 16 / 4 heads of 128, bf16.)
+// makes uneven.)
+// 16-bit types: S and dP of a wavefront's NEXT step are formed (matrix pipe) beside the exponentials of the present one, so rows
+// are copied two steps ahead into three buffers.  At D > 64 K, V, dK and dV take 192 registers per lane: one wavefront per SIMD,
+// which hides latency by that order alone.
+template <typename T, int DK>
+constexpr bool kv_ahead() {
+  return sizeof(T) == 2;
+}
+template <typename T, int DK>
+constexpr int kv_lds() {
+  constexpr int tiles = (kv_ahead<T, DK>() ? 6 : 4) * 64 * lds_width(DK) * (int)sizeof(T), join = 2 * 32 * DK * 4;
+  return tiles > join ? tiles : join;
+}
 template <typename T, int DK, bool DROP>
 __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_kv(Args a) {
   constexpr int W = lds_width(DK), BM = 64;
+  constexpr bool kAhead = kv_ahead<T, DK>();
+  constexpr int NB = kAhead ? 3 : 2;
   typedef Tile<T, W> TL;
   typedef PackedPipe<T, W, BM> Pipe;
-  extern __shared__ __attribute__((aligned(16))) char lds[];      // [2][2][kTileBytes]: Q and dO of two steps
-  __shared__ __attribute__((aligned(16))) float row_lse[2][BM], row_delta[2][BM];
-  __shared__ __attribute__((aligned(16))) int row_lim[2][BM];
+  extern __shared__ __attribute__((aligned(16))) char lds[];      // [NB][2][kTileBytes]: Q and dO of NB steps
+  __shared__ __attribute__((aligned(16))) float row_lse[NB][BM], row_delta[NB][BM];
+  __shared__ __attribute__((aligned(16))) int row_lim[NB][BM];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
   const int kg = wave & 1, part = wave >> 1;
   const Work wk = causal_order((int)blockIdx.x, a.n_tiles, a.B * a.Hk, a.cus_per_xcd);
@@ -178,35 +168,62 @@ __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_
   const Pipe qp(a, a.q, b, hk, r_end, tid), dop(a, a.dout, b, hk, r_end, tid);
   auto tile_at = [&](int buf, int which) { return lds + (2 * buf + which) * Pipe::kTileBytes; };
   if (a.D < W)
-    for (int i = 0; i < 4; ++i) qp.clear(lds + i * Pipe::kTileBytes);
-  float st_lse = 0.0f, st_delta = 0.0f;
-  int st_lim = 0;
+    for (int i = 0; i < 2 * NB; ++i) qp.clear(lds + i * Pipe::kTileBytes);
+  float st_lse = 0.0f, st_delta = 0.0f;      // (asked for before the copies and looked at when those have arrived)
   auto issue = [&](int m0, int buf) {
+    if (tid < BM) {
+      const int64_t r = (int64_t)unit * a.R + min(m0 + tid, r_end - 1);
+      st_lse = a.lse[r], st_delta = a.delta[r];
+    }
     qp.issue(m0, tile_at(buf, 0));
     dop.issue(m0, tile_at(buf, 1));
-    if (tid < BM) {
-      const int r = m0 + tid;
-      const bool ok = r < r_end;
-      st_lse = ok ? a.lse[(int64_t)unit * a.R + r] * kLog2e : 0.0f;
-      st_delta = ok ? a.delta[(int64_t)unit * a.R + r] : 0.0f;
-      st_lim = ok ? row_limit(a, n, row_query(a, r)) : 0;
-    }
   };
-  if (r_begin < r_end) issue(r_begin, 0);
-  int buf = 0;
-  for (int m0 = r_begin; m0 < r_end; m0 += BM, buf ^= 1) {
+  auto arrive = [&](int m0, int buf) {      // (a barrier must follow)
     copies_done();
     if (m0 + BM > r_end) qp.hide(tile_at(buf, 0), m0), dop.hide(tile_at(buf, 1), m0);
-    if (tid < BM) row_lse[buf][tid] = st_lse, row_delta[buf][tid] = st_delta, row_lim[buf][tid] = st_lim;
-    __syncthreads();
-    if (m0 + BM < r_end) issue(m0 + BM, buf ^ 1);
+    if (tid < BM) {
+      const bool ok = m0 + tid < r_end;
+      row_lse[buf][tid] = ok ? st_lse * kLog2e : 0.0f, row_delta[buf][tid] = ok ? st_delta : 0.0f;
+      row_lim[buf][tid] = ok ? row_limit(a, n, row_query(a, m0 + tid)) : 0;
+    }
+  };
+  const int o0 = 32 * part;
+  f32x16 s = {}, dp = {};
+  auto products = [&](int buf, f32x16& x, f32x16& y) {
+    x = f32x16{}, y = f32x16{};
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) x = mma(TL::row(tile_at(buf, 0), o0 + col, t, hi), kf[t], x);
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) y = mma(TL::row(tile_at(buf, 1), o0 + col, t, hi), vf[t], y);
+  };
+  if (r_begin < r_end) {
+    issue(r_begin, 0);
+    if (kAhead) {
+      arrive(r_begin, 0);
+      __syncthreads();
+      if (r_begin + BM < r_end) issue(r_begin + BM, 1);
+      products(0, s, dp);
+    }
+  }
+  int buf = 0;
+  for (int m0 = r_begin; m0 < r_end; m0 += BM) {
+    const int buf1 = buf + 1 == NB ? 0 : buf + 1, buf2 = buf1 + 1 == NB ? 0 : buf1 + 1;
+    if (kAhead) {      // rows of the next step
+      if (m0 + BM < r_end) arrive(m0 + BM, buf1);
+      __syncthreads();
+      if (m0 + 2 * BM < r_end) issue(m0 + 2 * BM, buf2);
+    } else {
+      arrive(m0, buf);
+      __syncthreads();
+      if (m0 + BM < r_end) issue(m0 + BM, buf1);
+      products(buf, s, dp);
+    }
     const char *qt = tile_at(buf, 0), *dot = tile_at(buf, 1);
-    const int o0 = 32 * part;
-    f32x16 s = {}, dp = {};
-#pragma unroll
-    for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(qt, o0 + col, t, hi), kf[t], s);
-#pragma unroll
-    for (int t = 0; t < DK / 16; ++t) dp = mma(TL::row(dot, o0 + col, t, hi), vf[t], dp);
+    // rows see more keys the later they are: no masks when the step's first row sees the wavefront's last key
+    const bool masked = m0 + BM > r_end || (a.causal && row_lim[buf][o0] < key0 + kg * 32 + 32);
+    // (behind the last step: products of whatever the buffer holds, never looked at)
+    f32x16 s1, dp1;
+    if (kAhead) products(buf1, s1, dp1);
     uint32_t w[4];
     if (DROP) drop_words_keys(seed, (uint32_t)unit, m0 + o0, key, lane, w);
 #pragma unroll
@@ -223,9 +240,8 @@ __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_
         dp[g] = p * (dpv - delta[c]);
       }
     }
-    // rows see more keys the later they are: no masks when the step's first row sees the wavefront's last key
-    if (m0 + BM > r_end || (a.causal && row_lim[buf][o0] < key0 + kg * 32 + 32)) {
-      asm volatile("");
+    if (masked) {
+      asm volatile("");      // (a branch, not a select per score)
 #pragma unroll
       for (int g = 0; g < 16; ++g) {
         const bool see = key < row_lim[buf][o0 + 8 * (g >> 2) + 4 * hi + (g & 3)];
@@ -241,6 +257,8 @@ __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_
         dk[dt] = mma(TL::col(qt, o0 + 16 * t, dt, lane), ds, dk[dt]);
       }
     }
+    if (kAhead) s = s1, dp = dp1;
+    buf = buf1;
   }
   // the odd steps' sums into the even steps' wavefronts: (register, lane) by (register, lane)
   __syncthreads();
@@ -410,7 +428,8 @@ int launch(const Args& a0, hipStream_t st) {
   }
   a.n_tiles = ceil_div(a.Lk, 64);
   if (units * a.n_tiles >= (1ll << 31)) return PSTL_ERR_SHAPE;
-  constexpr int kBytes = 4 * 64 * lds_width(DK) * (int)sizeof(T) > 2 * 32 * DK * 4 ? 4 * 64 * lds_width(DK) * (int)sizeof(T) : 2 * 32 * DK * 4;
+  if (waves_per_simd_kv<T, DK>() == 1) a.cus_per_xcd = 1 << 24;      // one workgroup per compute unit
+  constexpr int kBytes = kv_lds<T, DK>();
   if (int e = allow_lds<k_attn_bwd_kv<T, DK, DROP>>(kBytes)) return e;
   hipLaunchKernelGGL((k_attn_bwd_kv<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), kBytes, st, a);
   return launch_status();

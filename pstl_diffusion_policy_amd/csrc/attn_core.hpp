@@ -109,8 +109,8 @@ __device__ inline float half_sum(float x) {
 
 // ---- LDS tiles ----------------------------------------------------------------------------------------------------
 // A tile of rows of W elements (a power of two) is stored row after row in 16-byte chunks; chunk c of row r sits at position
-// c ^ swz(r).  Rows 0..15 then put the same chunk on different banks (row fragments), and so do the four rows that a transposing
-// 16-bit read takes together (column fragments).
+// c ^ swz(r).  Rows 0..15 then put the same chunk on different banks (row fragments), and the four rows x 64 bytes that half a
+// wavefront takes in one transposing 16-bit read lie on 64 different ones (column fragments).
 template <typename T, int W>
 struct Tile {
   static constexpr int kChunkEl = 16 / (int)sizeof(T);
@@ -118,8 +118,8 @@ struct Tile {
   static constexpr int kRowBytes = W * (int)sizeof(T);
   __device__ static inline int swz(int r) {
     if constexpr (kChunks == 4) return (r >> 2) & 3;
-    if constexpr (kChunks == 8) return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
-    return ((r & 7) << 1) | ((r >> 3) & 1);
+    if constexpr (kChunks == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    return ((r & 3) << 2) | ((r >> 2) & 3);
   }
   __device__ static inline int chunk_off(int r, int c) { return r * kRowBytes + ((c ^ swz(r)) << 4); }
   // row fragment: row `r`, elements 16 t + 8 hi + 0..7
@@ -274,12 +274,13 @@ __device__ inline int xcd_order(int x, int n) {
 }
 
 // Order of the workgroups of a causal launch.  All tiles of a unit stay on one XCD (or on 8 / units of them); inside an XCD the
-// longest come first, and every second round of one tile per compute unit runs backwards, so that the two workgroups a compute
-// unit holds at once are a long and a short one.  Where the units do not divide the XCDs evenly: xcd_order, longest first.
+// longest come first, and every second round of `round` tiles runs backwards: with two workgroups on a compute unit at once
+// (round = compute units of an XCD) they are a long and a short one; with one (round past the grid) the next free unit takes the
+// longest that is left.  Where the units do not divide the XCDs evenly: xcd_order, longest first.
 struct Work {
   int unit, tile;
 };
-__device__ inline Work causal_order(int x, int n_tiles, int units, int cus_per_xcd) {
+__device__ inline Work causal_order(int x, int n_tiles, int units, int round_len) {
   const int total = n_tiles * units, xcd = x & 7, q = x >> 3;
   int share = 0;                      // XCDs that share a unit's tiles
   if (units % 8 == 0) share = 1;
@@ -288,8 +289,8 @@ __device__ inline Work causal_order(int x, int n_tiles, int units, int cus_per_x
     const int w = xcd_order(x, total), unit = w / n_tiles;
     return Work{unit, n_tiles - 1 - (w - unit * n_tiles)};
   }
-  const int per = total >> 3, round = q / cus_per_xcd, i = q - round * cus_per_xcd, width = min(cus_per_xcd, per - round * cus_per_xcd);
-  const int pos = round * cus_per_xcd + ((round & 1) ? width - 1 - i : i);
+  const int per = total >> 3, round = q / round_len, i = q - round * round_len, width = min(round_len, per - round * round_len);
+  const int pos = round * round_len + ((round & 1) ? width - 1 - i : i);
   const int here = share > 1 ? 1 : units >> 3, u = pos % here;      // units of this XCD
   return share > 1 ? Work{xcd / share, n_tiles - 1 - (pos * share + xcd % share)} : Work{xcd * here + u, n_tiles - 1 - pos / here};
 }

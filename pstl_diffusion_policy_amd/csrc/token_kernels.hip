@@ -21,11 +21,12 @@ struct RopeArgs {
   const double* freq;
   float* part;                       // (workgroups, 2, D) sums of dz o xhat
   int heads[2];
-  int L, D, rot, pairs, lanes, lane_shift, interleaved, per_block;
-  int64_t tokens;
-  float eps;
+  uint32_t head_magic[2];            // x / heads = umulhi(x, magic) for heads > 1 (x heads < 2^32: kRopeTokens and the heads are bounded)
+  int L, D, rot, pairs, lanes, lane_shift, interleaved, per_block, tokens;
+  float eps, inv_d;
 };
 constexpr int kRopeTable = 2048;     // (cos, sin) entries of a workgroup
+constexpr int kRopeTokens = 32;      // tokens of a workgroup and iteration, at most
 
 template <typename T>
 __device__ inline f32x8 up8(const T* p) {
@@ -43,26 +44,38 @@ __device__ inline void down8(T* p, f32x8 v) {
 }
 __device__ inline void rotate(f32x8& a, f32x8& b, const float2* cs, const RopeArgs& p, int chunk, float sign) {
   if (p.interleaved) {
-    const float2 *c0 = cs + 4 * chunk, *c1 = c0 + (p.rot >> 2);
+    const f32x4 *c0 = reinterpret_cast<const f32x4*>(cs + 4 * chunk), *c1 = reinterpret_cast<const f32x4*>(cs + 4 * chunk + (p.rot >> 2));
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const float2 u = c0[m], v = c1[m];
-      const float a0 = a[2 * m], a1 = a[2 * m + 1], b0 = b[2 * m], b1 = b[2 * m + 1], us = sign * u.y, vs = sign * v.y;
-      a[2 * m] = a0 * u.x - a1 * us, a[2 * m + 1] = a1 * u.x + a0 * us;
-      b[2 * m] = b0 * v.x - b1 * vs, b[2 * m + 1] = b1 * v.x + b0 * vs;
+      const f32x4 uu = c0[m >> 1], vv = c1[m >> 1];
+      const float ux = uu[2 * (m & 1)], us = sign * uu[2 * (m & 1) + 1], vx = vv[2 * (m & 1)], vs = sign * vv[2 * (m & 1) + 1];
+      const float a0 = a[2 * m], a1 = a[2 * m + 1], b0 = b[2 * m], b1 = b[2 * m + 1];
+      a[2 * m] = a0 * ux - a1 * us, a[2 * m + 1] = a1 * ux + a0 * us;
+      b[2 * m] = b0 * vx - b1 * vs, b[2 * m + 1] = b1 * vx + b0 * vs;
     }
   } else {
-    const float2* c0 = cs + 8 * chunk;
+    const f32x4* c0 = reinterpret_cast<const f32x4*>(cs + 8 * chunk);
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
-      const float2 u = c0[m];
-      const float a0 = a[m], b0 = b[m], us = sign * u.y;
-      a[m] = a0 * u.x - b0 * us, b[m] = b0 * u.x + a0 * us;
+      const f32x4 uu = c0[m >> 1];
+      const float ux = uu[2 * (m & 1)], us = sign * uu[2 * (m & 1) + 1];
+      const float a0 = a[m], b0 = b[m];
+      a[m] = a0 * ux - b0 * us, b[m] = b0 * ux + a0 * us;
     }
   }
 }
+// sum over the `lanes` (1, 2, ... 32) neighbouring lanes of a head.  Inside a row of 16 by DPP: once the sums of 2, 4, 8 lanes are
+// equal in their groups, mirroring a group of 4, 8, 16 brings the other half's.
+template <int CTRL>
+__device__ inline float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
 __device__ inline float lanes_sum(float v, int lanes) {
-  for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o);
+  if (lanes > 1) v = dpp_add<0xB1>(v);       // quad_perm [1,0,3,2]
+  if (lanes > 2) v = dpp_add<0x4E>(v);       // quad_perm [2,3,0,1]
+  if (lanes > 4) v = dpp_add<0x141>(v);      // row_half_mirror
+  if (lanes > 8) v = dpp_add<0x140>(v);      // row_mirror
+  if (lanes > 16) v += __shfl_xor(v, 16);
   return v;
 }
 __device__ inline float dot8(f32x8 a, f32x8 b) {
@@ -73,9 +86,12 @@ __device__ inline float dot8(f32x8 a, f32x8 b) {
 }
 
 template <typename T, bool BWD>
-__global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs p) {
-  __shared__ float2 table[kRopeTable];
-  __shared__ float sums[4][64][17];
+__global__ __launch_bounds__(256, 4) void k_qk_norm_rope(RopeArgs p) {
+  __shared__ __attribute__((aligned(16))) char lds[BWD ? 4 * 32 * 17 * 4 : kRopeTable * 8];
+  __shared__ __attribute__((aligned(16))) float weight[2][PSTL_ROPE_MAX_D];
+  __shared__ int2 place[kRopeTokens];      // (sequence, position in it) of the iteration's tokens
+  float2* table = reinterpret_cast<float2*>(lds);
+  static_assert(4 * 32 * 17 * 4 >= 1024 * 8, "the backward table fits");
   const int tid = threadIdx.x, half = p.rot >> 1;
   // a thread's place inside a head is the same in every iteration (256 is a multiple of `lanes`)
   const int c = tid & (p.lanes - 1);
@@ -83,49 +99,55 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs p) {
   const int d0 = pair ? 8 * c : p.rot + 8 * (c - p.pairs), d1 = d0 + half;
   const bool ok = d0 < p.D;
   const f32x8 zero = {};
-  f32x8 wa[2], wb[2], ga[2], gb[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    wa[s] = ok ? up8<float>(p.w[s] + d0) : zero;
-    wb[s] = ok && pair ? up8<float>(p.w[s] + d1) : zero;
-    ga[s] = zero, gb[s] = zero;
-  }
-  for (int64_t t0 = (int64_t)blockIdx.x * p.per_block; t0 < p.tokens; t0 += (int64_t)gridDim.x * p.per_block) {
-    const int nt = (int)min((int64_t)p.per_block, p.tokens - t0);
+  f32x8 ga = zero, gb = zero;
+  const int s_first = BWD ? (int)blockIdx.y : 0, s_end = BWD ? s_first + 1 : 2;      // (backward: queries or keys, one set of sums)
+  for (int s = s_first; s < s_end; ++s)
+    for (int d = tid; d < p.D; d += 256) weight[s][d] = p.w[s][d];
+  const int w0 = ok ? d0 : 0, w1 = ok && pair ? d1 : 0;      // (a lane without elements multiplies zeros)
+  for (int t0 = (int)blockIdx.x * p.per_block; t0 < p.tokens; t0 += (int)gridDim.x * p.per_block) {
+    const int nt = min(p.per_block, p.tokens - t0);
+    __syncthreads();
+    if (tid < nt) {
+      const int b = (t0 + tid) / p.L;
+      place[tid] = int2{b, t0 + tid - b * p.L};
+    }
     __syncthreads();
     for (int e = tid; e < nt * half; e += 256) {
       const int tt = e / half, i = e - tt * half;
-      const int64_t tok = t0 + tt, b = tok / p.L, l = tok - b * p.L;
-      const double rev = (double)p.pos[b * p.pos_sb + l] * (p.freq[i] * 0.15915494309189533577);
+      const int2 at = place[tt];
+      const double rev = (double)p.pos[at.x * p.pos_sb + at.y] * (p.freq[i] * 0.15915494309189533577);
       const float x = 2.0f * (float)(rev - __builtin_rint(rev));
       table[e] = float2{cospif(x), sinpif(x)};
     }
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = s_first; s < s_end; ++s) {
       const int H = p.heads[s], n = (nt * H) << p.lane_shift;
       for (int u = tid; u < n; u += 256) {
-        const int th = u >> p.lane_shift, tt = th / H, h = th - tt * H;
-        const int64_t tok = t0 + tt, b = tok / p.L, l = tok - b * p.L;
-        const T* x = reinterpret_cast<const T*>(p.x[s].p) + b * p.x[s].sb + l * p.x[s].sl + h * p.x[s].sh;
+        const int th = u >> p.lane_shift, tt = H == 1 ? th : (int)__umulhi((uint32_t)th, p.head_magic[s]), h = th - tt * H;
+        const int2 at = place[tt];
+        const T* x = reinterpret_cast<const T*>(p.x[s].p) + at.x * p.x[s].sb + at.y * p.x[s].sl + h * p.x[s].sh;
         f32x8 a = ok ? up8<T>(x + d0) : zero, bb = ok && pair ? up8<T>(x + d1) : zero;
+        f32x8 za, zb;
+        if (BWD) {
+          const T* dy = reinterpret_cast<const T*>(p.dy[s].p) + at.x * p.dy[s].sb + at.y * p.dy[s].sl + h * p.dy[s].sh;
+          za = ok ? up8<T>(dy + d0) : zero, zb = ok && pair ? up8<T>(dy + d1) : zero;
+        }
         const float ss = lanes_sum(dot8(a, a) + dot8(bb, bb), p.lanes);
-        const float rstd = 1.0f / __builtin_sqrtf(ss / (float)p.D + p.eps);
+        const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, p.inv_d, p.eps));      // (one step of 2^-23)
         a *= rstd, bb *= rstd;
         if (!BWD) {
-          a *= wa[s], bb *= wb[s];
+          a *= up8<float>(&weight[s][w0]), bb *= up8<float>(&weight[s][w1]);
           if (pair) rotate(a, bb, table + tt * half, p, c, 1.0f);
-          T* y = reinterpret_cast<T*>(p.y[s].p) + b * p.y[s].sb + l * p.y[s].sl + h * p.y[s].sh;
+          T* y = reinterpret_cast<T*>(p.y[s].p) + at.x * p.y[s].sb + at.y * p.y[s].sl + h * p.y[s].sh;
           if (ok) down8<T>(y + d0, a);
           if (ok && pair) down8<T>(y + d1, bb);
         } else {
-          const T* dy = reinterpret_cast<const T*>(p.dy[s].p) + b * p.dy[s].sb + l * p.dy[s].sl + h * p.dy[s].sh;
-          f32x8 za = ok ? up8<T>(dy + d0) : zero, zb = ok && pair ? up8<T>(dy + d1) : zero;
           if (pair) rotate(za, zb, table + tt * half, p, c, -1.0f);
-          ga[s] += za * a, gb[s] += zb * bb;
-          za *= wa[s], zb *= wb[s];
-          const float mean = lanes_sum(dot8(za, a) + dot8(zb, bb), p.lanes) / (float)p.D;
-          T* dx = reinterpret_cast<T*>(p.dx[s].p) + b * p.dx[s].sb + l * p.dx[s].sl + h * p.dx[s].sh;
+          ga += za * a, gb += zb * bb;
+          za *= up8<float>(&weight[s][w0]), zb *= up8<float>(&weight[s][w1]);
+          const float mean = lanes_sum(dot8(za, a) + dot8(zb, bb), p.lanes) * p.inv_d;
+          T* dx = reinterpret_cast<T*>(p.dx[s].p) + at.x * p.dx[s].sb + at.y * p.dx[s].sl + h * p.dx[s].sh;
           if (ok) down8<T>(dx + d0, (za - a * mean) * rstd);
           if (ok && pair) down8<T>(dx + d1, (zb - bb * mean) * rstd);
         }
@@ -134,26 +156,24 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope(RopeArgs p) {
   }
   if (BWD) {      // sums of the workgroup, in a fixed order: over the lanes of a wavefront that share a place, then the wavefronts
     const int lane = tid & 63, wave = tid >> 6;
+    float(*sums)[32][17] = reinterpret_cast<float(*)[32][17]>(lds);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        for (int o = p.lanes; o < 64; o <<= 1) {
-          ga[s][j] += __shfl_xor(ga[s][j], o);
-          gb[s][j] += __shfl_xor(gb[s][j], o);
-        }
-      __syncthreads();
-      if (lane < p.lanes)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sums[wave][lane][j] = ga[s][j], sums[wave][lane][8 + j] = gb[s][j];
-      __syncthreads();
-      for (int e = tid; e < p.lanes * 16; e += 256) {
-        const int lc = e >> 4, j = e & 15, second = j >> 3;
-        const bool lp = lc < p.pairs;
-        const int d = (lp ? 8 * lc + second * half : p.rot + 8 * (lc - p.pairs)) + (j & 7);
-        if (d >= p.D || (second && !lp)) continue;
-        p.part[((int64_t)blockIdx.x * 2 + s) * p.D + d] = sums[0][lc][j] + sums[1][lc][j] + sums[2][lc][j] + sums[3][lc][j];
+    for (int j = 0; j < 8; ++j)
+      for (int o = p.lanes; o < 64; o <<= 1) {
+        ga[j] += __shfl_xor(ga[j], o);
+        gb[j] += __shfl_xor(gb[j], o);
       }
+    __syncthreads();
+    if (lane < p.lanes)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[wave][lane][j] = ga[j], sums[wave][lane][8 + j] = gb[j];
+    __syncthreads();
+    for (int e = tid; e < p.lanes * 16; e += 256) {
+      const int lc = e >> 4, j = e & 15, second = j >> 3;
+      const bool lp = lc < p.pairs;
+      const int d = (lp ? 8 * lc + second * half : p.rot + 8 * (lc - p.pairs)) + (j & 7);
+      if (d >= p.D || (second && !lp)) continue;
+      p.part[((int64_t)blockIdx.x * 2 + s_first) * p.D + d] = sums[0][lc][j] + sums[1][lc][j] + sums[2][lc][j] + sums[3][lc][j];
     }
   }
 }
@@ -183,12 +203,13 @@ __global__ __launch_bounds__(1024) void k_qk_norm_rope_dw(const float* part, int
   }
 }
 
+constexpr int kRopeMaxBlocks = 2048;
 int rope_args(const pstl_qk_rope* c, RopeArgs* p, bool backward) {
   if (!c) return PSTL_ERR_ARG;
   if (c->dtype != PSTL_F32 && c->dtype != PSTL_BF16 && c->dtype != PSTL_F16) return PSTL_ERR_SHAPE;
   if (c->B < 0 || c->L < 0 || c->Hq < 1 || c->Hk < 1 || !(c->eps >= 0.0f)) return PSTL_ERR_ARG;
   if (c->D < 8 || c->D > PSTL_ROPE_MAX_D || c->D % 8 || c->rot < 16 || c->rot > c->D || c->rot % 16) return PSTL_ERR_SHAPE;
-  if (c->Hq > 65536 || c->Hk > 65536) return PSTL_ERR_SHAPE;
+  if (c->Hq > 8192 || c->Hk > 8192) return PSTL_ERR_SHAPE;
   *p = RopeArgs();
   const int el = c->dtype == PSTL_F32 ? 4 : 2;
   const bool any = (int64_t)c->B * c->L > 0;
@@ -211,18 +232,21 @@ int rope_args(const pstl_qk_rope* c, RopeArgs* p, bool backward) {
   p->pairs = c->rot / 16;
   const int need = p->pairs + (c->D - c->rot) / 8;
   while (p->lanes = 1 << p->lane_shift, p->lanes < need) ++p->lane_shift;
-  p->tokens = (int64_t)c->B * c->L;
+  if ((int64_t)c->B * c->L >= (1ll << 30)) return PSTL_ERR_SHAPE;      // (32-bit tokens)
+  p->tokens = c->B * c->L;
+  auto magic = [](int d) { return d > 1 ? (uint32_t)((1ull << 32) / (uint64_t)d + 1) : 0u; };
+  p->head_magic[0] = magic(c->Hq), p->head_magic[1] = magic(c->Hk);
+  p->inv_d = 1.0f / (float)c->D;
   return PSTL_OK;
 }
-constexpr int kRopeMaxBlocks = 2048;
-// workgroups and tokens per workgroup and iteration: one token each while that does not fill the chip, else a few, so that the
-// angles' table is shared by at least two iterations of the heads' loop
+// workgroups and tokens per workgroup and iteration: one token each while that does not fill the chip, else as many as give every
+// thread a few heads, so that the angles' table and the barriers around it are shared
 void rope_grid(RopeArgs* p, int* blocks) {
-  const int units = (p->heads[0] + p->heads[1]) << p->lane_shift;
+  const int units = (p->heads[0] + p->heads[1]) << p->lane_shift, table = 1024;
   int per = 1;
-  while (per < 32 && per * units < 1024 && p->tokens > (int64_t)per * 2 * kRopeMaxBlocks && 2 * per * (p->rot / 2) <= kRopeTable) per *= 2;
+  while (per < kRopeTokens && per * units < 2048 && p->tokens > per * 2 * kRopeMaxBlocks && 2 * per * (p->rot / 2) <= table) per *= 2;
   p->per_block = per;
-  const int64_t n = (p->tokens + per - 1) / per;
+  const int64_t n = ((int64_t)p->tokens + per - 1) / per;
   *blocks = (int)(n < kRopeMaxBlocks ? n : kRopeMaxBlocks);
 }
 
@@ -297,7 +321,7 @@ int rope_launch(RopeArgs& p, bool backward, float* dwq, float* dwk, hipStream_t 
   rope_grid(&p, &blocks);
   if (blocks > 0) {
     if (backward)
-      hipLaunchKernelGGL((k_qk_norm_rope<T, true>), dim3(blocks), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((k_qk_norm_rope<T, true>), dim3(blocks, 2), dim3(256), 0, st, p);
     else
       hipLaunchKernelGGL((k_qk_norm_rope<T, false>), dim3(blocks), dim3(256), 0, st, p);
     if (int e = launch_status()) return e;

@@ -298,11 +298,18 @@ __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_
 }
 
 // ---- at most 32 keys: one wavefront per (sequence, key head), or per pair of them, everything in one pass ------------------
-// K and V stay in the LDS, rows come 32 at a time; delta is the row sum of P o m dP / keep, so that O is not read.  S and dP are
-// formed in both layouts (a product more against a transposition through the LDS).  Bound by memory, as the forward kernel.
-template <typename T, int DK, bool DROP, bool PAIR>
-__global__ __launch_bounds__(64 * (short_waves<T, DK>(4))) void k_attn_bwd_short(Args a) {
-  constexpr int NW = short_waves<T, DK>(4);
+// K and V stay in the LDS, rows come 32 at a time; delta is the row sum of P o m dP / keep, so that O is not read.  dK and dV need P
+// and dS with a key per lane: 16-bit types form S and dP a second time in that layout; float32, whose products take sixteen times
+// as long, turns P and dS through the LDS when there is one row tile (their tiles take the places of V and K).
+template <typename T, int DK>
+constexpr int bwd_short_waves() {
+  return DK <= 32 ? 2 : short_waves<T, DK>(4);
+}
+// ONE: at most 32 rows
+template <typename T, int DK, bool DROP, bool PAIR, bool ONE>
+__global__ __launch_bounds__(64 * (bwd_short_waves<T, DK>()), DK <= 64 ? 2 : 1) void k_attn_bwd_short(Args a) {
+  constexpr int NW = bwd_short_waves<T, DK>();
+  constexpr bool kTurn = sizeof(T) == 4 && ONE;
   typedef Rows32<T, DK> RW;
   constexpr int kTileBytes = 32 * RW::TL::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[NW][4][kTileBytes];
@@ -327,7 +334,7 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(4))) void k_attn_bwd_short
   const uint32_t keys_on = (uint32_t)__ballot(key_on);
   const uint64_t seed = DROP ? drop_seed(a) : 0;
   f32x16 dk[DK / 32] = {}, dv[DK / 32] = {};
-  for (int m0 = 0; m0 < a.R; m0 += 32) {
+  for (int m0 = 0; m0 < (ONE ? min(a.R, 1) : a.R); m0 += 32) {
     auto row_at = [&](const Mat& m) {
       return [&, m](int row) -> T* {
         const Slot s = slot_of<PAIR>(a, u0, units, row);
@@ -364,10 +371,25 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(4))) void k_attn_bwd_short
       s[g] = p, dp[g] = dpv;
     }
     delta = half_sum(delta);
+    f32x16 dq[DK / 32] = {};
+    if constexpr (kTurn) {
+      f32x16 pk;      // m P
+#pragma unroll
+      for (int g = 0; g < 16; ++g) {
+        pk[g] = !DROP || kept(w, g, a.thr) ? s[g] : 0.0f;
+        s[g] = s[g] * (dp[g] - delta);
+      }
+      Turned::put(vt, pk, lane);
+      contract<T, DK, PAIR>(dq, kt, s, lane);
+      wave_lds_fence();
+      Turned::put(kt, s, lane);
+      contract<T, DK, PAIR>(dv, dot, Turned::frag(vt, 0, lane), Turned::frag(vt, 1, lane), lane);
+      wave_lds_fence();
+      contract<T, DK, PAIR>(dk, qt, Turned::frag(kt, 0, lane), Turned::frag(kt, 1, lane), lane);
+    } else {
 #pragma unroll
     for (int g = 0; g < 16; ++g) s[g] = s[g] * (dp[g] - delta);
     if (hi == 0) row_stat[wave][0][col] = lse2, row_stat[wave][1][col] = delta, row_see[wave][col] = see;
-    f32x16 dq[DK / 32] = {};
     contract<T, DK, PAIR>(dq, kt, s, lane);
     wave_lds_fence();
     // keys in the lanes: dK, dV
@@ -391,6 +413,7 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(4))) void k_attn_bwd_short
     }
     contract<T, DK, PAIR>(dv, dot, s, lane);
     contract<T, DK, PAIR>(dk, qt, dp, lane);
+    }
     wave_lds_fence();
     RW::from_acc(qt, col, hi, dq, a.scale, live);
     wave_lds_fence();
@@ -410,14 +433,16 @@ int launch(const Args& a0, hipStream_t st) {
   a.cus_per_xcd = device_cus() >= 8 ? device_cus() / 8 : 1;
   const int64_t units = (int64_t)a.B * a.Hk;
   if (a.Lk <= 32) {
-    constexpr int NW = short_waves<T, DK>(4);
+    constexpr int NW = bwd_short_waves<T, DK>();
     const bool pair = in_pairs(a);
     const int64_t jobs = pair ? (units + 1) / 2 : units;
     const dim3 grid((unsigned)((jobs + NW - 1) / NW)), block(64 * NW);
     if (pair)
-      hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, true>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, true, true>), grid, block, 0, st, a);
+    else if (a.R <= 32)
+      hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, false, true>), grid, block, 0, st, a);
     else
-      hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, false>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, false, false>), grid, block, 0, st, a);
     return launch_status();
   }
   if (a.R > 0) {

@@ -159,17 +159,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK > 64 ? 1 : 2) void k_attn
 // neighbouring 16 bytes (fragments read straight from global memory touch 32 rows per instruction: 82 us instead of the 59 us of
 // this kernel at 4096 x 12 tokens, 8 heads of 32, float32).
 template <typename T, int DK, bool DROP, bool PAIR>
-__global__ __launch_bounds__(64 * (short_waves<T, DK>(3))) void k_attn_fwd_short(Args a) {
-  constexpr int NW = short_waves<T, DK>(3);
+__global__ __launch_bounds__(64 * (short_waves<T, DK>(2))) void k_attn_fwd_short(Args a) {
+  constexpr int NW = short_waves<T, DK>(2);
   typedef Rows32<T, DK> RW;
   constexpr int kTileBytes = 32 * RW::TL::kRowBytes;
-  __shared__ __attribute__((aligned(16))) char lds[NW][3][kTileBytes];
+  __shared__ __attribute__((aligned(16))) char lds[NW][2][kTileBytes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, col = lane & 31;
   const int units = a.B * a.Hk, groups = PAIR ? (units + 1) / 2 : units;
   const int job = (int)blockIdx.x * NW + wave;
   if (job >= groups * a.n_tiles) return;       // (no workgroup barrier below)
   const int group = job / a.n_tiles, tile = job - group * a.n_tiles, u0 = PAIR ? 2 * group : group;
-  char *kt = lds[wave][0], *vt = lds[wave][1], *qt = lds[wave][2];
+  char *kt = lds[wave][0], *qt = lds[wave][1];      // keys, then values; queries, then results
   // (loads are bounded by the tensors, not by the lengths and masks, so that they do not wait for those)
   RW kr, vr, qr;
   auto key_at = [&](const Mat& m) {
@@ -197,9 +197,10 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(3))) void k_attn_fwd_short
   const uint32_t see = seen_bits<PAIR>(keys_on, live ? row_limit(a, n, qi) : 0, lane) >> (4 * hi);
   kr.put(kt, keys_on, lane);
   qr.put(qt, rows_on, lane);
-  vr.put(vt, keys_on, lane);
   wave_lds_fence();
   f32x16 s = row_product<T, DK>(kt, qt, lane);
+  wave_lds_fence();
+  vr.put(kt, keys_on, lane);
   float mx = -INFINITY;
 #pragma unroll
   for (int g = 0; g < 16; ++g) {
@@ -221,7 +222,8 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(3))) void k_attn_fwd_short
     for (int g = 0; g < 16; ++g) s[g] = kept(w, g, a.thr) ? s[g] : 0.0f;
   }
   f32x16 acc[DK / 32] = {};
-  contract<T, DK, PAIR>(acc, vt, s, lane);
+  wave_lds_fence();
+  contract<T, DK, PAIR>(acc, kt, s, lane);
   const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : l;      // (0 for a row that sees nothing; a NaN sum stays one)
   if (hi == 0 && a.lse && me.ok && r < a.R)
     a.lse[(int64_t)me.unit * a.R + r] = live && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
@@ -422,7 +424,7 @@ int launch(const Args& a0, const FwdPlan& p, hipStream_t st) {
   if (p.kind == kManyRows) {
     hipLaunchKernelGGL((k_attn_fwd<T, DK, DROP>), dim3((unsigned)(units * p.n_tiles)), dim3(256), 0, st, a);
   } else if (p.kind == kShort || p.kind == kShortPairs) {
-    constexpr int NW = short_waves<T, DK>(3);
+    constexpr int NW = short_waves<T, DK>(2);
     const bool pair = p.kind == kShortPairs;
     const int64_t jobs = (pair ? (units + 1) / 2 : units) * p.n_tiles;
     const dim3 grid((unsigned)((jobs + NW - 1) / NW)), block(64 * NW);

@@ -525,11 +525,11 @@ struct Rows32 {
       }
   }
 };
-// sum over the tile's 32 slots of  A(slot) x f(slot):  acc[dt] (+)= columns of `tile` times the fragments of s; PAIR: the lane's half
+// sum over the tile's 32 slots of  A(slot) x f(slot):  acc[dt] += columns of `tile` times the fragments f0 (slots 0..15), f1; PAIR:
+// the lane's half
 template <typename T, int DK, bool PAIR>
-__device__ inline void contract(f32x16 (&acc)[DK / 32], const char* tile, const f32x16& s, int lane) {
+__device__ inline void contract(f32x16 (&acc)[DK / 32], const char* tile, const Frag<T>& f0, const Frag<T>& f1, int lane) {
   typedef Tile<T, lds_width(DK)> TL;
-  const Frag<T> f0 = acc_frag<T>(s, 0), f1 = acc_frag<T>(s, 1);
   const bool second = (lane & 16) != 0;
 #pragma unroll
   for (int dt = 0; dt < DK / 32; ++dt) {
@@ -543,6 +543,30 @@ __device__ inline void contract(f32x16 (&acc)[DK / 32], const char* tile, const 
     }
   }
 }
+template <typename T, int DK, bool PAIR>
+__device__ inline void contract(f32x16 (&acc)[DK / 32], const char* tile, const f32x16& s, int lane) {
+  contract<T, DK, PAIR>(acc, tile, acc_frag<T>(s, 0), acc_frag<T>(s, 1), lane);
+}
+// Float tile T[key][row] of 32 x 32 from an accumulator whose lanes are rows and registers keys; its row fragments then are the
+// contraction's operand for lanes that are keys (slots: rows)
+struct Turned {
+  typedef Tile<float, 32> TL;
+  __device__ static inline void put(char* tile, const f32x16& s, int lane) {
+    const int hi = lane >> 5, row = lane & 31;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) {
+      const int key = 8 * (g >> 2) + 4 * hi + (g & 3);
+      *reinterpret_cast<float*>(tile + TL::chunk_off(key, row >> 2) + (row & 3) * 4) = s[g];
+    }
+  }
+  // slots 0..3: rows 16 t + 4 hi + 0..3, slots 4..7: rows 16 t + 8 + 4 hi + 0..3 -- the order of Tile::col
+  __device__ static inline f32x8 frag(const char* tile, int t, int lane) {
+    const int hi = lane >> 5, key = lane & 31;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(tile + TL::chunk_off(key, 4 * t + hi));
+    const f32x4 b = *reinterpret_cast<const f32x4*>(tile + TL::chunk_off(key, 4 * t + 2 + hi));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
 // the tile's product over the element index: result(row i of x, lane = row of y)
 template <typename T, int DK>
 __device__ inline f32x16 row_product(const char* x, const char* y, int lane) {

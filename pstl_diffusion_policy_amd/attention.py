@@ -26,9 +26,10 @@ import torch
 from . import ffi
 
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+SHORT_KEYS = 32               # up to here one wavefront holds all keys: never a workspace
 MAX_HEAD_DIM = 128            # attention (include/pstl_hip.h, PSTL_ATTN_MAX_D)
 MAX_ROPE_HEAD_DIM = 256       # qk_norm_rope (PSTL_ROPE_MAX_D)
-_NO_MAT = (0, 0, 0, 0)
+_MASKS = (torch.bool, torch.uint8)
 # pstl_attn and pstl_qk_rope as bytes (ffi.Attn, ffi.QkRope; a ctypes.Structure takes longer to fill than a small call runs)
 _ATTN = struct.Struct("@8ifiQQ32q6q")
 _ROPE = struct.Struct("@8ifi32q8q")
@@ -73,7 +74,15 @@ def _check_aligned(name, t):
 
 
 def _mat(t):
-    return (t.data_ptr(),) + t.stride()[:3]
+    sb, sl, sh, _ = t.stride()
+    return t.data_ptr(), sb, sl, sh
+
+
+def _good(t, like, el16):
+    """Is t (B, L, H, D) of `like`'s type and device, with rows the kernels can read 16 bytes at a time?"""
+    sb, sl, sh, sd = t.stride()
+    return (t.dtype is like.dtype and t.get_device() == like.get_device() and sd == 1 and not (sb | sl | sh) % el16
+            and not t.data_ptr() % 16)
 
 
 def _ptr(t):
@@ -102,22 +111,6 @@ def _seed(seed, device):
     return seed & (2 ** 64 - 1), None
 
 
-class _on_device:
-    """The operands' device as the current one, if it is not already."""
-    __slots__ = ("guard",)
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
 def _once(backward):
     """torch.autograd.function.once_differentiable (a second derivative raises), entered only when a graph of the backward pass is
     asked for."""
@@ -129,7 +122,22 @@ def _once(backward):
 
 
 def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if getattr(t, "requires_grad", False):
+                return True
+    return False
+
+
+def _device_guard(launch):
+    """launch(q, ...) with q's device as the current one, if it is not already."""
+    def run(q, *args):
+        index = q.get_device()
+        if index == torch.cuda.current_device():
+            return launch(q, *args)
+        with torch.cuda.device(index):
+            return launch(q, *args)
+    return run
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -143,6 +151,25 @@ def rope_frequencies(rot_dim, base=10000.0, device=None):
 
 
 def _rope_checks(q, k, q_weight, k_weight, positions, inv_freq, eps):
+    try:      # everything at once; what is wrong, and how to say it, below
+        B, L, Hq, D = q.shape
+        dev, el16 = q.get_device(), 4 if q.dtype is torch.float32 else 8
+        if (q.dtype in _CODES and dev >= 0 and k.shape[0] == B and k.shape[1] == L and k.shape[2] > 0 and Hq > 0 and k.shape[3] == D
+                and not D % 8 and 8 <= D <= MAX_ROPE_HEAD_DIM and _good(q, q, el16) and _good(k, q, el16)
+                and q_weight.dtype is torch.float32 and k_weight.dtype is torch.float32 and q_weight.shape == (D,) == k_weight.shape
+                and q_weight.get_device() == dev == k_weight.get_device() and q_weight.is_contiguous() and k_weight.is_contiguous()
+                and not (q_weight.data_ptr() | k_weight.data_ptr()) % 16
+                and positions.dtype is torch.int64 and positions.get_device() == dev and positions.is_contiguous()
+                and (positions.shape == (B, L) or positions.shape == (L,))
+                and inv_freq.dtype is torch.float64 and inv_freq.get_device() == dev and inv_freq.is_contiguous() and inv_freq.dim() == 1
+                and not inv_freq.numel() % 8 and 16 <= 2 * inv_freq.numel() <= D and eps >= 0.0):
+            return
+    except (AttributeError, TypeError, ValueError, IndexError):
+        pass
+    _rope_diagnose(q, k, q_weight, k_weight, positions, inv_freq, eps)
+
+
+def _rope_diagnose(q, k, q_weight, k_weight, positions, inv_freq, eps):
     if not eps >= 0.0:
         raise ValueError("eps must not be negative, got %r" % (eps,))
     _rows("q", q)
@@ -176,34 +203,41 @@ def _rope_checks(q, k, q_weight, k_weight, positions, inv_freq, eps):
             raise ValueError("%s must be 16-byte aligned" % name)
 
 
-def _rope_launch(q, k, wq, wk, positions, inv_freq, eps, interleaved, grads=None):
-    """The call on checked operands; grads = (dyq, dyk): the backward pass."""
+_rope_work = {}      # head dimension -> floats of workspace
+
+
+@_device_guard
+def _rope_launch(q, k, wq, wk, positions, inv_freq, eps, interleaved, dyq=None, dyk=None):
+    """The call on checked operands; with the gradients of its outputs: the backward pass."""
     B, L, Hq, D = q.shape
+    Hk = k.shape[2]
     dev = q.device
-    with _on_device(dev):
-        yq, yk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))      # forward's results, or the gradients of q and k
-        if grads is None:
-            mats, tail = _mat(yq) + _mat(yk) + 4 * _NO_MAT, (0, 0, 0)
-        else:
-            dyq, dyk = _gradient(grads[0], q), _gradient(grads[1], k)
-            dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
-            mats = 2 * _NO_MAT + _mat(dyq) + _mat(dyk) + _mat(yq) + _mat(yk)
-            tail = (dwq.data_ptr(), dwk.data_ptr(), 0)
-        head = (_CODES[q.dtype], B, L, Hq, k.shape[2], D, 2 * inv_freq.numel(), 1 if interleaved else 0, eps, 0) + _mat(q) + _mat(k)
-        mid = (wq.data_ptr(), wk.data_ptr(), positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
-               inv_freq.data_ptr())
-        lib = ffi.lib()
-        a = _ROPE.pack(*head, *mats, *mid, *tail)
-        if grads is None:
-            rc = lib.pstl_qk_norm_rope(a, _raw_stream(dev.index))
-            if rc:
-                ffi.check(rc, "qk_norm_rope")
-            return yq, yk
-        work = torch.empty(lib.pstl_qk_norm_rope_work_floats(a), dtype=torch.float32, device=dev)
-        rc = lib.pstl_qk_norm_rope_backward(_ROPE.pack(*head, *mats, *mid, *tail[:2], work.data_ptr()), _raw_stream(dev.index))
+    out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)      # forward's results, or the gradients of q and k
+    out_k = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    oq, ok = (out_q.data_ptr(), L * Hq * D, Hq * D, D), (out_k.data_ptr(), L * Hk * D, Hk * D, D)
+    pos_stride = L if positions.dim() == 2 else 0
+    lib, stream = ffi.lib(), _raw_stream(dev.index)
+    if dyq is None:
+        rc = lib.pstl_qk_norm_rope(_ROPE.pack(
+            _CODES[q.dtype], B, L, Hq, Hk, D, 2 * inv_freq.numel(), 1 if interleaved else 0, eps, 0, *_mat(q), *_mat(k), *oq, *ok,
+            0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, wq.data_ptr(), wk.data_ptr(), positions.data_ptr(), pos_stride,
+            inv_freq.data_ptr(), 0, 0, 0), stream)
         if rc:
-            ffi.check(rc, "qk_norm_rope_backward")
-        return yq, yk, dwq, dwk
+            ffi.check(rc, "qk_norm_rope")
+        return out_q, out_k
+    dyq, dyk = _gradient(dyq, q), _gradient(dyk, k)
+    dwq = torch.empty(D, dtype=torch.float32, device=dev)
+    dwk = torch.empty(D, dtype=torch.float32, device=dev)
+    if D not in _rope_work:
+        _rope_work[D] = lib.pstl_qk_norm_rope_work_floats(bytes(ffi.QkRope(D=D)))
+    work = torch.empty(_rope_work[D], dtype=torch.float32, device=dev)
+    rc = lib.pstl_qk_norm_rope_backward(_ROPE.pack(
+        _CODES[q.dtype], B, L, Hq, Hk, D, 2 * inv_freq.numel(), 1 if interleaved else 0, eps, 0, *_mat(q), *_mat(k),
+        0, 0, 0, 0, 0, 0, 0, 0, *_mat(dyq), *_mat(dyk), *oq, *ok, wq.data_ptr(), wk.data_ptr(), positions.data_ptr(), pos_stride,
+        inv_freq.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), work.data_ptr()), stream)
+    if rc:
+        ffi.check(rc, "qk_norm_rope_backward")
+    return out_q, out_k, dwq, dwk
 
 
 def qk_norm_rope_forward(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
@@ -218,7 +252,7 @@ def qk_norm_rope_backward(dyq, dyk, q, k, q_weight, k_weight, positions, inv_fre
     for name, t, x in (("dyq", dyq, q), ("dyk", dyk, k)):
         if t.shape != x.shape or t.device != x.device:
             raise ValueError("%s must be %s on %s" % (name, tuple(x.shape), x.device))
-    return _rope_launch(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, (dyq, dyk))
+    return _rope_launch(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved, dyq, dyk)
 
 
 class _QkNormRope(torch.autograd.Function):
@@ -232,7 +266,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dyq, dyk):
-        return _rope_launch(*ctx.saved_tensors, *ctx.opts, (dyq, dyk)) + (None,) * 4
+        return _rope_launch(*ctx.saved_tensors, *ctx.opts, dyq, dyk) + (None,) * 4
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
@@ -252,6 +286,27 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
 # ---------------------------------------------------------------------------------------------------------------
 def _attn_checks(q, k, v, key_mask, q_lens, k_lens, dropout_p):
     """Checks the operands; returns the dropout probability in 256ths."""
+    try:      # everything at once; what is wrong, and how to say it, below
+        B, Lq, Hq, D = q.shape
+        Bk, Lk, Hk, _ = shape = k.shape
+        dev, el16 = q.get_device(), 4 if q.dtype is torch.float32 else 8
+        n256 = int(round(256 * dropout_p))
+        if (q.dtype in _CODES and dev >= 0 and Bk == B and shape[3] == D and v.shape == shape and Hk > 0 and Hq > 0 and not Hq % Hk
+                and not D % 8 and 8 <= D <= MAX_HEAD_DIM and _good(q, q, el16) and _good(k, q, el16) and _good(v, q, el16)
+                and (dropout_p == 0.0 or 1 <= n256 <= 255)
+                and (key_mask is None or (key_mask.dtype in _MASKS and key_mask.get_device() == dev and key_mask.shape == (B, Lk)
+                                          and key_mask.is_contiguous()))
+                and (q_lens is None or (q_lens.dtype is torch.int32 and q_lens.shape == (B,) and q_lens.get_device() == dev
+                                        and q_lens.is_contiguous()))
+                and (k_lens is None or (k_lens.dtype is torch.int32 and k_lens.shape == (B,) and k_lens.get_device() == dev
+                                        and k_lens.is_contiguous()))):
+            return n256
+    except (AttributeError, TypeError, ValueError, IndexError):
+        pass
+    return _attn_diagnose(q, k, v, key_mask, q_lens, k_lens, dropout_p)
+
+
+def _attn_diagnose(q, k, v, key_mask, q_lens, k_lens, dropout_p):
     _rows("q", q)
     _rows("k", k, q)
     _rows("v", v, q)
@@ -296,44 +351,48 @@ def _attn_scale(scale, D):
     return scale
 
 
+@_device_guard
 def _attn_forward(q, k, v, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev, need_lse):
     """The call on checked operands: (out, lse or None)."""
     B, Lq, Hq, D = q.shape
     Lk, Hk = k.shape[1], k.shape[2]
     dev = q.device
-    with _on_device(dev):
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        lse = torch.empty((B, Hk, Lq, Hq // Hk), dtype=torch.float32, device=dev) if need_lse else None
-        head = (_CODES[q.dtype], B, Lq, Lk, Hq, Hk, D, 1 if causal else 0, scale, n256, seed, _ptr(seed_dev)) + _mat(q) + _mat(k) \
-            + _mat(v) + _mat(out) + 4 * _NO_MAT
-        tail = (_ptr(lse), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _ptr(q_lens), _ptr(k_lens))
-        lib = ffi.lib()
-        a = _ATTN.pack(*head, *tail, 0)
-        n = lib.pstl_attention_work_floats(a) if Lk > 32 else 0      # (a split call: few rows, many keys)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Hk, Lq, Hq // Hk), dtype=torch.float32, device=dev) if need_lse else None
+    head = (_CODES[q.dtype], B, Lq, Lk, Hq, Hk, D, 1 if causal else 0, scale, n256, seed, _ptr(seed_dev), *_mat(q), *_mat(k), *_mat(v),
+            out.data_ptr(), Lq * Hq * D, Hq * D, D, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, _ptr(lse), _ptr(key_mask),
+            0 if key_mask is None else key_mask.stride(0), _ptr(q_lens), _ptr(k_lens))
+    lib = ffi.lib()
+    a = _ATTN.pack(*head, 0)
+    if Lk > SHORT_KEYS:      # (few rows against many keys: the call may be split)
+        n = lib.pstl_attention_work_floats(a)
         if n:
             work = torch.empty(n, dtype=torch.float32, device=dev)
-            a = _ATTN.pack(*head, *tail, work.data_ptr())
-        rc = lib.pstl_attention(a, _raw_stream(dev.index))
-        if rc:
-            ffi.check(rc, "attention")
+            a = _ATTN.pack(*head, work.data_ptr())
+    rc = lib.pstl_attention(a, _raw_stream(dev.index))
+    if rc:
+        ffi.check(rc, "attention")
     return out, lse
 
 
-def _attn_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev):
+@_device_guard
+def _attn_backward(q, k, v, dout, out, lse, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev):
     """The call on checked operands: (dq, dk, dv)."""
     B, Lq, Hq, D = q.shape
-    dev = q.device
-    with _on_device(dev):
-        dout = _gradient(dout, q)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        head = (_CODES[q.dtype], B, Lq, k.shape[1], Hq, k.shape[2], D, 1 if causal else 0, scale, n256, seed, _ptr(seed_dev)) \
-            + _mat(q) + _mat(k) + _mat(v) + _mat(out) + _mat(dout) + _mat(dq) + _mat(dk) + _mat(dv) \
-            + (lse.data_ptr(), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _ptr(q_lens), _ptr(k_lens))
-        lib = ffi.lib()
-        work = torch.empty(lib.pstl_attention_backward_work_floats(_ATTN.pack(*head, 0)), dtype=torch.float32, device=dev)
-        rc = lib.pstl_attention_backward(_ATTN.pack(*head, work.data_ptr()), _raw_stream(dev.index))
-        if rc:
-            ffi.check(rc, "attention_backward")
+    Lk, Hk = k.shape[1], k.shape[2]
+    dev, dtype = q.device, q.dtype
+    dout = _gradient(dout, q)
+    dq = torch.empty(q.shape, dtype=dtype, device=dev)
+    dk = torch.empty(k.shape, dtype=dtype, device=dev)
+    dv = torch.empty(k.shape, dtype=dtype, device=dev)
+    work = torch.empty(B * Hq * Lq + 1, dtype=torch.float32, device=dev)      # pstl_attention_backward_work_floats
+    rc = ffi.lib().pstl_attention_backward(_ATTN.pack(
+        _CODES[dtype], B, Lq, Lk, Hq, Hk, D, 1 if causal else 0, scale, n256, seed, _ptr(seed_dev), *_mat(q), *_mat(k), *_mat(v),
+        *_mat(out), *_mat(dout), dq.data_ptr(), Lq * Hq * D, Hq * D, D, dk.data_ptr(), Lk * Hk * D, Hk * D, D, dv.data_ptr(),
+        Lk * Hk * D, Hk * D, D, lse.data_ptr(), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _ptr(q_lens),
+        _ptr(k_lens), work.data_ptr()), _raw_stream(dev.index))
+    if rc:
+        ffi.check(rc, "attention_backward")
     return dq, dk, dv
 
 
@@ -359,7 +418,7 @@ def attention_backward(dout, q, k, v, out, lse, causal=False, key_mask=None, q_l
             or lse.device != q.device):
         raise ValueError("out (%s) and lse (float32, %s) are what attention_forward returned" % (q.dtype, (B, Hk, Lq, Hq // Hk)))
     _check_aligned("out", out)
-    return _attn_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, _attn_scale(scale, q.shape[3]), n256,
+    return _attn_backward(q, k, v, dout, out, lse, causal, key_mask, q_lens, k_lens, _attn_scale(scale, q.shape[3]), n256,
                           *_seed(seed, q.device))
 
 
@@ -383,7 +442,7 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dout, *_):
         q, k, v, out, lse, key_mask, q_lens, k_lens, seed_dev = ctx.saved_tensors
         causal, scale, n256, seed = ctx.opts
-        return _attn_backward(dout, q, k, v, out, lse, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev) + (None,) * 8
+        return _attn_backward(q, k, v, dout, out, lse, causal, key_mask, q_lens, k_lens, scale, n256, seed, seed_dev) + (None,) * 8
 
 
 def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, scale=None, dropout_p=0.0, seed=0,
@@ -416,18 +475,18 @@ def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, sc
 # ---------------------------------------------------------------------------------------------------------------
 # dropout
 # ---------------------------------------------------------------------------------------------------------------
+@_device_guard
 def _dropout_launch(x, residual, p, value, seed_dev, offset):
-    dev = x.device
-    with _on_device(dev):
-        if not x.is_contiguous():
-            x = x.contiguous()
-        if residual is not None and not residual.is_contiguous():
-            residual = residual.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        rc = ffi.lib().pstl_dropout_add(_CODES[x.dtype], x.numel(), x.data_ptr(), _ptr(residual), y.data_ptr(), int(round(65536 * p)),
-                                        value - 2 ** 64 if value >= 2 ** 63 else value, _ptr(seed_dev), offset, _raw_stream(dev.index))
-        if rc:
-            ffi.check(rc, "dropout_add")
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if residual is not None and not residual.is_contiguous():
+        residual = residual.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rc = ffi.lib().pstl_dropout_add(_CODES[x.dtype], x.numel(), x.data_ptr(), _ptr(residual), y.data_ptr(), int(round(65536 * p)),
+                                    value - 2 ** 64 if value >= 2 ** 63 else value, _ptr(seed_dev), offset,
+                                    _raw_stream(x.get_device()))
+    if rc:
+        ffi.check(rc, "dropout_add")
     return y
 
 

@@ -201,6 +201,18 @@ def test_c_entry_points_refuse_missing_buffers_and_accept_empty_calls():
     assert L.pstl_dropout_add(0, 0, None, None, None, 0, 0, None, 0, None) == 0
 
 
+def test_workspace_sizes_the_binding_takes_for_granted():
+    """attention.py asks for the backward workspace, and for none with few keys, without calling the library."""
+    from pstl_diffusion_policy_amd import attention as A
+    from pstl_diffusion_policy_amd import ffi
+    L = ffi.lib()
+    for B, Lq, Lk, Hq, Hk in ((1, 1, 1, 1, 1), (3, 17, 900, 12, 4), (2, 0, 5, 2, 2), (70000, 2, 32, 8, 2), (1, 5000, 32, 1, 1)):
+        a = c_attn(B=B, Lq=Lq, Lk=Lk, Hq=Hq, Hk=Hk, D=32)
+        assert L.pstl_attention_backward_work_floats(ctypes.byref(a)) == B * Hq * Lq + 1
+        if Lk <= A.SHORT_KEYS:
+            assert L.pstl_attention_work_floats(ctypes.byref(a)) == 0
+
+
 @pytest.mark.parametrize("B, Lq, Lk, Hq, Hk, D", [(1, 1, 1, 1, 1, 8), (4096, 12, 12, 8, 8, 32), (4, 1, 32768, 16, 2, 128), (1, 5, 1 << 29, 8, 1, 64),
                                                   (1, 1 << 20, 1 << 20, 8, 8, 128), (65536, 1, 33, 64, 8, 64), (3, 100, 65, 6, 3, 80)])
 def test_split_calls_cover_every_key_with_bounded_work(B, Lq, Lk, Hq, Hk, D):

@@ -246,8 +246,8 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];       // 4 x kWaveBytes
   __shared__ float stat[4][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, col = lane & 31;
-  const int work = xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const int job = work / a.splits, split = work - job * a.splits;
+  // (in the grid's order: a sequence's parts go to all XCDs, so that short sequences leave none of them idle)
+  const int job = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - job * a.splits;
   const int unit = job / a.n_tiles, tile = job - unit * a.n_tiles;
   const int b = unit / a.Hk, hk = unit - b * a.Hk;
   const Lens n = lens_of(a, b);
@@ -321,19 +321,22 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(Args a) {
   const float f = __builtin_amdgcn_exp2f(m - (mj == -INFINITY ? 0.0f : mj));
   if (hi == 0) stat[wave][1][col] = l * f;
   float* part = reinterpret_cast<float*>(lds + wave * kWaveBytes);
+  const int rows = min(a.R - tile * 32, 32);
+  if (col < rows) {
 #pragma unroll
-  for (int dt = 0; dt < DK / 32; ++dt)
+    for (int dt = 0; dt < DK / 32; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f32x4 v;
+      for (int g = 0; g < 4; ++g) {
+        f32x4 v;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = acc[dt][4 * g + c] * f;
-      *reinterpret_cast<f32x4*>(part + col * DK + 32 * dt + 8 * g + 4 * hi) = v;
-    }
+        for (int c = 0; c < 4; ++c) v[c] = acc[dt][4 * g + c] * f;
+        *reinterpret_cast<f32x4*>(part + col * DK + 32 * dt + 8 * g + 4 * hi) = v;
+      }
+  }
   __syncthreads();
-  for (int e = tid; e < 32 * (DK / 4); e += 256) {
+  for (int e = tid; e < rows * (DK / 4); e += 256) {
     const int row = e / (DK / 4), d = (e - row * (DK / 4)) * 4, rr = tile * 32 + row;
-    if (rr >= a.R || d >= a.D) continue;
+    if (d >= a.D) continue;
     f32x4 v = {};
     float ls = 0.0f, mr = -INFINITY;
 #pragma unroll

@@ -89,8 +89,11 @@ inline FwdPlan plan_forward(const Args& a, int cus) {
   p.kind = kFewRows;
   p.n_tiles = ceil_div(a.R, 32);
   const int64_t jobs = units * p.n_tiles;
-  const int key_tiles = ceil_div(a.Lk, 32), most = ceil_div(key_tiles, 4);
-  const int64_t want = jobs >= cus ? 1 : (2 * cus + jobs - 1) / jobs;
+  // a part has at least 8 tiles (two per wavefront), and up to 16 tiles are not divided at all: joining costs a launch of 4 us
+  const int key_tiles = ceil_div(a.Lk, 32), most = key_tiles <= 16 ? 1 : ceil_div(key_tiles, 8);
+  // one workgroup per compute unit: its four wavefronts keep 64 KB of keys and values in flight; more workgroups only add
+  // starts and joins (4 x 32768 keys, 16 / 2 heads of 128, fp16: 1, 2, 3, 4 per unit took 30, 35, 42, 45 us)
+  const int64_t want = jobs >= cus ? 1 : cus / jobs;
   p.splits = (int)(want < most ? want : most);
   if (p.splits > kMaxSplits) p.splits = kMaxSplits;
   p.tiles_per_split = ceil_div(ceil_div(key_tiles, p.splits), 4) * 4;

@@ -54,11 +54,15 @@ def _rows(name, t, like=None):
             raise ValueError("%s is on %s, the queries are on %s" % (name, t.device, like.device))
 
 
+def _strides(t):
+    """Strides of sequence, position and head; that of a dimension of size 1 means nothing and is left out."""
+    return [0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride())]
+
+
 def _aligned(t):
     """Can the kernels read t's rows 16 bytes at a time?"""
     el = t.element_size()
-    sb, sl, sh, sd = t.stride()
-    return sd == 1 and t.data_ptr() % 16 == 0 and (sb * el) % 16 == 0 and (sl * el) % 16 == 0 and (sh * el) % 16 == 0
+    return t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(st * el % 16 for st in _strides(t))
 
 
 def _on_gpu(*tensors):
@@ -75,6 +79,8 @@ def _check_aligned(name, t):
 
 def _mat(t):
     sb, sl, sh, _ = t.stride()
+    if (sb | sl | sh) & 7:
+        sb, sl, sh = _strides(t)
     return t.data_ptr(), sb, sl, sh
 
 
@@ -215,7 +221,7 @@ def _rope_launch(q, k, wq, wk, positions, inv_freq, eps, interleaved, dyq=None, 
     out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)      # forward's results, or the gradients of q and k
     out_k = torch.empty(k.shape, dtype=q.dtype, device=dev)
     oq, ok = (out_q.data_ptr(), L * Hq * D, Hq * D, D), (out_k.data_ptr(), L * Hk * D, Hk * D, D)
-    pos_stride = L if positions.dim() == 2 else 0
+    pos_stride = positions.stride(0) if positions.dim() == 2 else 0
     lib, stream = ffi.lib(), _raw_stream(dev.index)
     if dyq is None:
         rc = lib.pstl_qk_norm_rope(_ROPE.pack(

@@ -100,6 +100,8 @@ def test_scale_seed_and_layout_checks():
     assert not A._aligned(torch.zeros(2, 3, 4, 12, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="contiguous"):
         A._check_aligned("q", base[..., 4:12])
+    one = torch.zeros(200).as_strided((1, 4, 1, 16), (3, 16, 5, 1))      # strides of dimensions of size 1 mean nothing
+    assert one.is_contiguous() and A._aligned(one) and A._mat(one)[1:] == (0, 16, 0)
     g = torch.ones((), dtype=torch.bfloat16).expand(2, 3, 4, 24)     # what sum().backward() hands over
     assert A._aligned(A._gradient(g, base))
     assert A._aligned(A._gradient(base.flatten()[4:52].view(1, 1, 6, 8), base))

@@ -78,6 +78,11 @@ __device__ inline float lanes_sum(float v, int lanes) {
   if (lanes > 16) v += __shfl_xor(v, 16);
   return v;
 }
+// 1 / sqrt(v): v_rsq_f32 (good to a step) and one Newton step; an overflowed sum of squares keeps its 0
+__device__ inline float inv_sqrt(float v) {
+  const float r = __builtin_amdgcn_rsqf(v), e = __builtin_fmaf(-v * r, r, 1.0f);
+  return v < INFINITY ? __builtin_fmaf(0.5f * r, e, r) : r;
+}
 __device__ inline float dot8(f32x8 a, f32x8 b) {
   float s = 0.0f;
 #pragma unroll
@@ -134,7 +139,7 @@ __global__ __launch_bounds__(256, 4) void k_qk_norm_rope(RopeArgs p) {
           za = ok ? up8<T>(dy + d0) : zero, zb = ok && pair ? up8<T>(dy + d1) : zero;
         }
         const float ss = lanes_sum(dot8(a, a) + dot8(bb, bb), p.lanes);
-        const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, p.inv_d, p.eps));      // (one step of 2^-23)
+        const float rstd = inv_sqrt(__builtin_fmaf(ss, p.inv_d, p.eps));
         a *= rstd, bb *= rstd;
         if (!BWD) {
           a *= up8<float>(&weight[s][w0]), bb *= up8<float>(&weight[s][w1]);

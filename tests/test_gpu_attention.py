@@ -368,21 +368,16 @@ def test_qk_norm_rope_positions_and_views():
     """Positions as an expanded row, as a column of a wider table, alone; (B, H, L, D) operands; one token of each sequence."""
     from pstl_diffusion_policy_amd import attention as A
     g = torch.Generator().manual_seed(3)
-    B, L, D = 3, 6, 32
+    B, D = 3, 32
     f, w = A.rope_frequencies(D), 1 + 0.1 * torch.randn(D, generator=g)
     table = torch.randint(0, 90000, (B, 40), generator=g)
-    for L, pos in ((6, table[:, 3:9]), (6, table[:1, :6].expand(B, 6)), (6, table[0, 1:7]), (1, table[:, 7:8]), (1, table[0, :1]), (6, table[:, ::1][:, :6])):
+    views = [(6, lambda t: t[:, 3:9]), (6, lambda t: t[:1, :6].expand(B, 6)), (6, lambda t: t[0, 1:7]), (1, lambda t: t[:, 7:8]),
+             (1, lambda t: t[0, :1])]
+    for L, view in views:
         x = torch.randn(B, 4, L, D, generator=g)
-        on = lambda t: t.to(DEV)
-        dev_pos = on(table)
-        dev_pos = (dev_pos[:, 3:9] if pos.dim() == 2 and torch.equal(pos, table[:, 3:9]) else pos.to(DEV))
-        if pos.dim() == 2 and pos.stride(0) == 0:
-            dev_pos = on(table)[:1, :6].expand(B, 6)
-        if L == 1 and pos.dim() == 2:
-            dev_pos = on(table)[:, 7:8]
-        q = x.transpose(1, 2)
-        yq, yk = A.qk_norm_rope(on(x).transpose(1, 2), on(x).transpose(1, 2)[:, :, 1:3], on(w), on(w), dev_pos, on(f))
-        res = ao.qk_norm_rope(q, w, pos, f)
+        q, xg = x.transpose(1, 2), x.to(DEV).transpose(1, 2)
+        yq, yk = A.qk_norm_rope(xg, xg[:, :, 1:3], w.to(DEV), w.to(DEV), view(table.to(DEV)), f.to(DEV))
+        res = ao.qk_norm_rope(q, w, view(table), f)
         tol = ao.half_step(torch.float32) * res["y"].abs() + (D + 16) * ao.E32 * res["mag"]
         within("yq", yq, res["y"], tol)
         within("yk", yk, res["y"][:, :, 1:3], tol[:, :, 1:3])

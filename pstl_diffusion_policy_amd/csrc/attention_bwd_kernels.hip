@@ -3,8 +3,8 @@
 //   P = exp(S - lse);  delta_r = sum_d dO_rd O_rd;  dV = (m P / keep)^T dO;  dP = dO V^T;  dS = P o (m dP / keep - delta)
 //   dQ = scale dS K;   dK = scale dS^T Q
 // Two launches without atomics, so that a result does not depend on the order in which workgroups finish: k_attn_bwd_q (a lane
-// holds one row: S^T, dP^T, dQ^T; it also leaves delta) and k_attn_bwd_kv (a lane holds one key: S, dP, dK^T, dV^T; packed rows
-// make the sum over the heads that share a key head part of the same accumulator).  S and dP are formed in both: seven products
+// holds one row: S^T, dP^T, dQ^T; it also leaves delta) and k_attn_bwd_kv or _kv_duo (a lane holds one key: S, dP, dK^T, dV^T;
+// packed rows make the sum over the heads that share a key head part of the same accumulator).  S and dP are formed in both: seven products
 // instead of five, against a second pass over dQ in memory.  Sequences of at most 32 keys have one launch (k_attn_bwd_short).
 // Arithmetic: P and dS are rounded to the inputs' type as operands of dV, dQ and dK; all sums are 32-bit.
 #include "attn_host.hpp"
@@ -23,7 +23,7 @@ constexpr int waves_per_simd_q() {
 }
 template <typename T, int DK>
 constexpr int waves_per_simd_kv() {
-  return sizeof(T) == 2 && DK <= 64 ? 2 : DK <= 32 ? 2 : 1;
+  return sizeof(T) == 2 || DK <= 32 ? 2 : 1;
 }
 
 // sum over d of the product of two rows (row fragments; both lane halves)
@@ -38,6 +38,11 @@ __device__ inline float row_dot(const Frag<T> (&x)[DK / 16], const Frag<T> (&y)[
 }
 
 // ---- dQ: 128 packed rows per workgroup, 32 per wavefront ---------------------------------------------------------------
+// Q, dO and dQ stay in registers, keys and values pass through the LDS as in the forward kernel; 16-bit types run two wavefronts
+// per SIMD, so that one's matrix products stand beside the other's exponentials (one per SIMD with the scores formed a step ahead:
+// 212 us).  4 x 2048 causal, 16/4 heads of 128, bf16: 134 us, 103 GF = 770 TF; the matrix pipe is busy 42 % of the time and the
+// vector pipe 34 %, the rest is LDS latency and the barrier of a tile.  (Copies asked for behind the products instead of right
+// behind the barrier: 135 us.)
 template <typename T, int DK, bool DROP>
 __global__ __launch_bounds__(256, (waves_per_simd_q<T, DK>())) void k_attn_bwd_q(Args a) {
   constexpr int W = lds_width(DK), BN = block_len<T>(), NS = BN / 32;
@@ -123,12 +128,13 @@ __global__ __launch_bounds__(256, (waves_per_simd_q<T, DK>())) void k_attn_bwd_q
 }
 
 // ---- dK, dV: 64 keys per workgroup --------------------------------------------------------------------------------------
+// float32, and 16-bit types up to D = 64.
 // Wavefronts 0, 1 take 32 keys each and the even 32-row steps, wavefronts 2, 3 the same keys and the odd steps; their sums are
 // joined in the LDS at the end.  (128 keys per workgroup, all steps in every wavefront: half the workgroups, which a causal mask
 // makes uneven.)
 // 16-bit types: S and dP of a wavefront's NEXT step are formed (matrix pipe) beside the exponentials of the present one, so rows
-// are copied two steps ahead into three buffers.  At D > 64 K, V, dK and dV take 192 registers per lane: one wavefront per SIMD,
-// which hides latency by that order alone.
+// are copied two steps ahead into three buffers.  4 x 2048 causal, 16/4 heads of 64, bf16: 219 us with dQ (k_attn_bwd_kv_duo
+// 226); heads of 128, float32: 2.18 ms with dQ, 241 GF = 110 of the 153 TF that a large float32 product reaches here.
 template <typename T, int DK>
 constexpr bool kv_ahead() {
   return sizeof(T) == 2;
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_
   const int key = key0 + kg * 32 + col;
   const bool live = key < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + key] != 0);
   const int r_end = key0 < n.k ? n.q * a.G : 0;
-  const int r_begin = a.causal ? max(key0 - (n.k - n.q), 0) * a.G / BM * BM : 0;
+  const int r_begin = a.causal && r_end > 0 ? max(key0 - (n.k - n.q), 0) * a.G / BM * BM : 0;
 
   Frag<T> kf[DK / 16], vf[DK / 16];
   load_row_frags<T, DK>(live ? key_ptr<T>(a.k, b, hk, key) : nullptr, live, a.D, hi, kf);
@@ -297,10 +303,176 @@ __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_
   store_col<T, DK>(key_ptr<T>(a.dv, b, hk, key), a.D, hi, dv, DROP ? a.keep_inv : 1.0f);
 }
 
+// 16-bit types, D > 64: K, V, dK and dV of 32 keys take 192 registers per lane, which leaves one wavefront per SIMD.  Here eight
+// wavefronts share them: 4 + w forms S, P and dV of 32 keys and every second 32-row step, and hands P (32 bits; the sign bit
+// marks a dropped probability) through the LDS to w on the same SIMD, which forms dP, dS and dK.  The second kind passes its
+// barrier between dP and dS, the first before S: one is in the matrix pipe while the other forms exponentials.  Copies are asked
+// for behind the first product: 32 KB take 500 cycles to issue, which right behind the barrier nobody had anything to do in.
+// 4 x 2048 causal, 16/4 heads of 128, bf16: 204 us, 137 GF = 670 TF (one wavefront per SIMD with all four: 241 us; both kinds
+// forming S for themselves: 245 us; copies right behind the barrier: 219 us; columns of Q and dO read ahead of the exponentials:
+// no gain).  At D <= 64 everything fits two wavefronts per SIMD in k_attn_bwd_kv, and the handing over only costs (219 -> 226 us).
+template <typename T, int DK>
+constexpr int kv_duo_lds() {
+  return 6 * 64 * lds_width(DK) * (int)sizeof(T) + 2 * 4 * 4096;
+}
+template <typename T, int DK, bool DROP>
+__global__ __launch_bounds__(512, 2) void k_attn_bwd_kv_duo(Args a) {
+  constexpr int W = lds_width(DK), BM = 64;
+  typedef Tile<T, W> TL;
+  typedef PackedPipe<T, W, BM> Pipe;
+  static_assert(4 * (DK / 32) * 4096 <= 6 * Pipe::kTileBytes, "the sums are joined in the tiles' place");
+  extern __shared__ __attribute__((aligned(16))) char lds[];      // [3][2][kTileBytes]: Q and dO of three steps; [2][4][4096]: P
+  __shared__ __attribute__((aligned(16))) float row_lse[3][BM], row_delta[3][BM];
+  __shared__ __attribute__((aligned(16))) int row_lim[3][BM];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+  const int kg = wave & 1, part = (wave >> 1) & 1, first = wave >> 2;      // first: S, P, dV; else dP, dS, dK
+  const Work wk = causal_order((int)blockIdx.x, a.n_tiles, a.B * a.Hk, a.cus_per_xcd);
+  const int unit = wk.unit, key0 = (a.n_tiles - 1 - wk.tile) * 64;      // (causal: the first keys are seen by the most rows)
+  const int b = unit / a.Hk, hk = unit - b * a.Hk;
+  const Lens n = lens_of(a, b);
+  const int key = key0 + kg * 32 + col;
+  const bool live = key < n.k && (!a.key_mask || a.key_mask[b * a.mask_sb + key] != 0);
+  const int r_end = key0 < n.k ? n.q * a.G : 0;
+  const int r_begin = a.causal && r_end > 0 ? max(key0 - (n.k - n.q), 0) * a.G / BM * BM : 0;
+
+  Frag<T> kv[DK / 16];      // this key's K or V
+  load_row_frags<T, DK>(live ? key_ptr<T>(first ? a.k : a.v, b, hk, key) : nullptr, live, a.D, hi, kv);
+  f32x16 acc[DK / 32] = {};
+  const uint64_t seed = DROP ? drop_seed(a) : 0;
+
+  const Pipe pipe(a, first ? a.dout : a.q, b, hk, r_end, tid & 255);      // each half of the workgroup copies one of the two
+  auto tile_at = [&](int buf, int which) { return lds + (2 * buf + which) * Pipe::kTileBytes; };
+  char* const p_at = lds + 6 * Pipe::kTileBytes + (wave & 3) * 4096 + lane * 16;
+  if (a.D < W)
+    for (int i = 0; i < 3; ++i) pipe.clear(tile_at(i, first));
+  float st_lse = 0.0f, st_delta = 0.0f;      // (asked for before the copies and looked at when those have arrived)
+  auto issue = [&](int m0, int buf) {
+    if (tid < BM) {
+      const int64_t r = (int64_t)unit * a.R + min(m0 + tid, r_end - 1);
+      st_lse = a.lse[r], st_delta = a.delta[r];
+    }
+    pipe.issue(m0, tile_at(buf, first));
+  };
+  const int o0 = 32 * part;
+  // makes step m0 visible
+  auto turn = [&](int m0, int buf) {
+    if (m0 < r_end) {
+      copies_done();
+      if (m0 + BM > r_end) pipe.hide(tile_at(buf, first), m0);
+      if (tid < BM) {
+        const bool ok = m0 + tid < r_end;
+        row_lse[buf][tid] = ok ? st_lse * kLog2e : 0.0f, row_delta[buf][tid] = ok ? st_delta : 0.0f;
+        row_lim[buf][tid] = ok ? row_limit(a, n, row_query(a, m0 + tid)) : 0;
+      }
+    }
+    __syncthreads();
+  };
+  if (r_begin < r_end) issue(r_begin, 0);
+  if (!first) {
+    turn(r_begin, 0);
+    if (r_begin + BM < r_end) issue(r_begin + BM, 1);
+  }
+  int buf = 0, slot = 0;
+  for (int m0 = r_begin; m0 < r_end; m0 += BM, slot ^= 4 * 4096) {
+    const int next = buf == 2 ? 0 : buf + 1;
+    if (first) turn(m0, buf);
+    f32x4 stat[4];      // lse or delta
+#pragma unroll
+    for (int q = 0; q < 4; ++q) stat[q] = *reinterpret_cast<const f32x4*>((first ? row_lse[buf] : row_delta[buf]) + o0 + 8 * q + 4 * hi);
+    f32x16 s = {};
+    const char* rows = tile_at(buf, 1 - first);
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) s = mma(TL::row(rows, o0 + col, t, hi), kv[t], s);      // S or dP
+    if (!first)
+      turn(m0 + BM, next);
+    else if (m0 + BM < r_end)
+      issue(m0 + BM, next);
+    // rows see more keys the later they are: no masks when the step's first row sees the wavefront's last key
+    const bool masked = m0 + BM > r_end || (a.causal && row_lim[buf][o0] < key0 + kg * 32 + 32);
+    uint32_t w[4];
+    if (first) {
+      if (DROP) drop_words_keys(seed, (uint32_t)unit, m0 + o0, key, lane, w);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[4 * q + c] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + c], a.c, -stat[q][c]));
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 p = *reinterpret_cast<const f32x4*>(p_at + slot + q * 1024);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x = p[c];
+          const float dpv = DROP ? (__builtin_signbitf(x) ? 0.0f : s[4 * q + c] * a.keep_inv) : s[4 * q + c];
+          s[4 * q + c] = (DROP ? __builtin_fabsf(x) : x) * (dpv - stat[q][c]);
+        }
+      }
+      if (m0 + 2 * BM < r_end) issue(m0 + 2 * BM, next == 2 ? 0 : next + 1);
+    }
+    if (masked) {
+      asm volatile("");      // (a branch, not a select per score; dS too: a row that does not see the key may hold anything)
+#pragma unroll
+      for (int g = 0; g < 16; ++g) s[g] = key < row_lim[buf][o0 + 8 * (g >> 2) + 4 * hi + (g & 3)] ? s[g] : 0.0f;
+    }
+    if (first) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4 p;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int g = 4 * q + c;
+          const bool keep = !DROP || kept(w, g, a.thr);
+          p[c] = keep ? s[g] : -s[g];
+          s[g] = keep ? s[g] : 0.0f;
+        }
+        *reinterpret_cast<f32x4*>(p_at + slot + q * 1024) = p;
+      }
+    }
+    const char* other = tile_at(buf, first);      // dV += dO^T P, dK += Q^T dS
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Frag<T> f = acc_frag<T>(s, t);
+#pragma unroll
+      for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = mma(TL::col(other, o0 + 16 * t, dt, lane), f, acc[dt]);
+    }
+    buf = next;
+  }
+  if (first) turn(r_end, 0);
+  // the odd steps' sums into the even steps' wavefronts: (register, lane) by (register, lane)
+  __syncthreads();
+  float* x = reinterpret_cast<float*>(lds) + (2 * first + kg) * (DK / 32) * 1024 + lane * 4;
+  if (part) {
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(x + dt * 1024 + q * 256) =
+            f32x4{acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]};
+  }
+  __syncthreads();
+  if (part || key >= a.Lk) return;
+#pragma unroll
+  for (int dt = 0; dt < DK / 32; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(x + dt * 1024 + q * 256);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[dt][4 * q + c] += y[c];
+    }
+  if (!live) {      // (a hidden key's column holds sums of no meaning, infinities among them: it is written as zeros)
+#pragma unroll
+    for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = f32x16{};
+  }
+  store_col<T, DK>(key_ptr<T>(first ? a.dv : a.dk, b, hk, key), a.D, hi, acc, !first ? a.scale : DROP ? a.keep_inv : 1.0f);
+}
+
 // ---- at most 32 keys: one wavefront per (sequence, key head), or per pair of them, everything in one pass ------------------
 // K and V stay in the LDS, rows come 32 at a time; delta is the row sum of P o m dP / keep, so that O is not read.  dK and dV need P
 // and dS with a key per lane: 16-bit types form S and dP a second time in that layout; float32, whose products take sixteen times
-// as long, turns P and dS through the LDS when there is one row tile (their tiles take the places of V and K).
+// as long, turns P and dS through the LDS when there is one row tile (their tiles take the places of V and K): 2048 x 20 tokens,
+// 8 heads of 32, float32, dropout: 112 us (formed twice: 128 us); 294 MB = 2.6 TB/s of 5.0, beside five products of 32 x 32 x 32
+// per unit, 5.4 GF = 35 us at the float32 matrix rate, and the exponentials and draws of 16384 tiles.
 template <typename T, int DK>
 constexpr int bwd_short_waves() {
   return DK <= 32 ? 2 : short_waves<T, DK>(4);
@@ -388,31 +560,31 @@ __global__ __launch_bounds__(64 * (bwd_short_waves<T, DK>()), DK <= 64 ? 2 : 1) 
       contract<T, DK, PAIR>(dk, qt, Turned::frag(kt, 0, lane), Turned::frag(kt, 1, lane), lane);
     } else {
 #pragma unroll
-    for (int g = 0; g < 16; ++g) s[g] = s[g] * (dp[g] - delta);
-    if (hi == 0) row_stat[wave][0][col] = lse2, row_stat[wave][1][col] = delta, row_see[wave][col] = see;
-    contract<T, DK, PAIR>(dq, kt, s, lane);
-    wave_lds_fence();
-    // keys in the lanes: dK, dV
-    s = row_product<T, DK>(qt, kt, lane), dp = row_product<T, DK>(dot, vt, lane);
-    if (DROP) drop_words_keys<PAIR>(seed, (uint32_t)me.unit, m0, me.at, lane, w);
+      for (int g = 0; g < 16; ++g) s[g] = s[g] * (dp[g] - delta);
+      if (hi == 0) row_stat[wave][0][col] = lse2, row_stat[wave][1][col] = delta, row_see[wave][col] = see;
+      contract<T, DK, PAIR>(dq, kt, s, lane);
+      wave_lds_fence();
+      // keys in the lanes: dK, dV
+      s = row_product<T, DK>(qt, kt, lane), dp = row_product<T, DK>(dot, vt, lane);
+      if (DROP) drop_words_keys<PAIR>(seed, (uint32_t)me.unit, m0, me.at, lane, w);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int o = 8 * q + 4 * hi;
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_stat[wave][0][o]), dl = *reinterpret_cast<const f32x4*>(&row_stat[wave][1][o]);
-      const u32x4v sees = *reinterpret_cast<const u32x4v*>(&row_see[wave][o]);
+      for (int q = 0; q < 4; ++q) {
+        const int o = 8 * q + 4 * hi;
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&row_stat[wave][0][o]), dl = *reinterpret_cast<const f32x4*>(&row_stat[wave][1][o]);
+        const u32x4v sees = *reinterpret_cast<const u32x4v*>(&row_see[wave][o]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int g = 4 * q + c;
-        const bool on = (sees[c] >> col) & 1;
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse[c]));
-        const bool keep = !DROP || kept(w, g, a.thr);
-        const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
-        s[g] = on && keep ? p : 0.0f;
-        dp[g] = on ? p * (dpv - dl[c]) : 0.0f;
+        for (int c = 0; c < 4; ++c) {
+          const int g = 4 * q + c;
+          const bool on = (sees[c] >> col) & 1;
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g], a.c, -lse[c]));
+          const bool keep = !DROP || kept(w, g, a.thr);
+          const float dpv = DROP ? (keep ? dp[g] * a.keep_inv : 0.0f) : dp[g];
+          s[g] = on && keep ? p : 0.0f;
+          dp[g] = on ? p * (dpv - dl[c]) : 0.0f;
+        }
       }
-    }
-    contract<T, DK, PAIR>(dv, dot, s, lane);
-    contract<T, DK, PAIR>(dk, qt, dp, lane);
+      contract<T, DK, PAIR>(dv, dot, s, lane);
+      contract<T, DK, PAIR>(dk, qt, dp, lane);
     }
     wave_lds_fence();
     RW::from_acc(qt, col, hi, dq, a.scale, live);
@@ -453,10 +625,18 @@ int launch(const Args& a0, hipStream_t st) {
   }
   a.n_tiles = ceil_div(a.Lk, 64);
   if (units * a.n_tiles >= (1ll << 31)) return PSTL_ERR_SHAPE;
-  if (waves_per_simd_kv<T, DK>() == 1) a.cus_per_xcd = 1 << 24;      // one workgroup per compute unit
-  constexpr int kBytes = kv_lds<T, DK>();
-  if (int e = allow_lds<k_attn_bwd_kv<T, DK, DROP>>(kBytes)) return e;
-  hipLaunchKernelGGL((k_attn_bwd_kv<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), kBytes, st, a);
+  const dim3 grid((unsigned)(units * a.n_tiles));
+  if constexpr (sizeof(T) == 2 && DK > 64) {
+    a.cus_per_xcd = 1 << 24;      // one workgroup per compute unit
+    constexpr int kBytes = kv_duo_lds<T, DK>();
+    if (int e = allow_lds<k_attn_bwd_kv_duo<T, DK, DROP>>(kBytes)) return e;
+    hipLaunchKernelGGL((k_attn_bwd_kv_duo<T, DK, DROP>), grid, dim3(512), kBytes, st, a);
+  } else {
+    if (waves_per_simd_kv<T, DK>() == 1) a.cus_per_xcd = 1 << 24;
+    constexpr int kBytes = kv_lds<T, DK>();
+    if (int e = allow_lds<k_attn_bwd_kv<T, DK, DROP>>(kBytes)) return e;
+    hipLaunchKernelGGL((k_attn_bwd_kv<T, DK, DROP>), grid, dim3(256), kBytes, st, a);
+  }
   return launch_status();
 }
 template <typename T, int DK>

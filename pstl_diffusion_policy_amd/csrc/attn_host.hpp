@@ -24,7 +24,7 @@ inline int attn_args(const pstl_attn* c, Args* a, Check what) {
   const int64_t G = c->Hq / c->Hk, R = (int64_t)c->Lq * G;
   // 32-bit row and key indexes with room for the tiles past the end, and the exact division of a row index by G
   if (R * G >= (1ll << 31) || R >= (1ll << 30) || c->Lk >= (1 << 30) || (int64_t)c->B * c->Hk >= (1ll << 30)) return PSTL_ERR_SHAPE;
-  if (!(c->scale > 0.0f) || !(c->scale < INFINITY)) return PSTL_ERR_ARG;
+  if (!(c->scale > 0.0f) || !(c->scale * kLog2e < INFINITY)) return PSTL_ERR_ARG;
   const int thr = c->dropout_256;
   if (thr < 0 || thr > 255) return PSTL_ERR_ARG;
   *a = Args();
@@ -84,6 +84,9 @@ inline FwdPlan plan_forward(const Args& a, int cus) {
     p.n_tiles = ceil_div(a.R, 32);
     return p;
   }
+  // up to 32 rows one wavefront's tile holds them all (128-row workgroups would leave three wavefronts idle and walk the keys one
+  // workgroup to a sequence).  Up to 256 rows and >= 1024 keys the 32-row kernel reads the keys up to eight times, from the L2, but
+  // spreads them over the chip: it is taken while the 128-row workgroups would fill less than half the compute units
   const bool few = a.R <= 32 || (units * p.n_tiles * 2 < cus && a.R <= 256 && a.Lk >= 1024);
   if (!few) return p;
   p.kind = kFewRows;

@@ -13,6 +13,9 @@ namespace {
 // half the rotated width apart, so that both pair orders are rotated inside the thread; `lanes` (a power of two) consecutive
 // lanes make a head.  The angles of a token are shared by all its heads: they are formed once per workgroup, in 64 bits and in
 // revolutions (pos f / 2 pi less its whole part), because a float32 angle of position 10^6 is off by 0.06 rad.
+// 4 x 4096 tokens, 20 heads of 128, bf16: forward 39 us (168 MB = 4.3 TB/s), backward 70 us (252 MB = 3.6 TB/s: its two sums per
+// head and the weights' gradients are vector work beside the loads); 4096 x 20 tokens, 16 heads of 32, float32: 39 and 56 us.
+// (Heads summed by shuffles through the LDS and queries' and keys' gradients in one workgroup: 43 and 93 us.)
 struct RopeArgs {
   Mat x[2], y[2], dy[2], dx[2];      // [0] queries, [1] keys
   const float* w[2];
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(256, 4) void k_qk_norm_rope(RopeArgs p) {
 }
 
 // dw[s][d] = sum over the workgroups' parts: one workgroup per (s, 32 elements), 32 strided sums each, joined in order.  Bound by
-// the latency of its loads: eight are in flight per thread (8 strided sums with one load in flight took 60 us for 2048 parts).
+// the latency of its loads: eight are in flight per thread, 2048 parts take 6 us (8 strided sums with one load in flight: 60 us).
 __global__ __launch_bounds__(1024) void k_qk_norm_rope_dw(const float* part, int blocks, int D, float* dwq, float* dwk) {
   __shared__ float s[32][32];
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, d = (int)blockIdx.x * 32 + lane, which = blockIdx.y;
@@ -257,7 +260,8 @@ void rope_grid(RopeArgs* p, int* blocks) {
 
 // ---- dropout + residual ------------------------------------------------------------------------------------------------
 //   y = residual + m x / keep,   m_n = [16 bits of philox((n + offset) / 8, 'DROP')  >=  65536 p]
-// Bound by memory; one draw of 128 bits serves eight elements.  A multiplication by the mask would turn a dropped infinity into
+// Bound by memory: 16384 x 1024, bf16, with residual: 101 MB in 20 us = 5.0 TB/s, the rate of a copy; backward 67 MB in 13 us.  One
+// draw of 128 bits serves eight elements.  A multiplication by the mask would turn a dropped infinity into
 // NaN: dropped elements are selected away.
 struct DropArgs {
   const void *x, *res;

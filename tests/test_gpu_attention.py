@@ -229,6 +229,24 @@ def test_offsets_past_32_bits():
         del base, gk, gv
 
 
+def test_more_than_2_31_packed_rows_of_keys_behind_the_length():
+    """Causal, 16 heads to a key head, a cache whose slots x heads pass 2^31 with five keys in it: the rest gets zeros."""
+    from pstl_diffusion_policy_amd import attention as A
+    Lk, G, D = 2 ** 27 + 4096, 16, 8
+    g = torch.Generator().manual_seed(5)
+    q, do = (torch.randn(1, 2, G, D, generator=g, dtype=torch.float32).to(DEV, torch.bfloat16) for _ in range(2))
+    k = torch.zeros(1, 1, 1, D, device=DEV, dtype=torch.bfloat16).expand(1, Lk, 1, D)      # (every slot the same memory)
+    kw = dict(causal=True, k_lens=torch.tensor([5], dtype=torch.int32, device=DEV))
+    out, lse = A.attention_forward(q, k, k, **kw)
+    dq, dk, dv = A.attention_backward(do, q, k, k, out, lse, **kw)
+    assert not dk[:, 5:].any() and not dv[:, 5:].any() and not out.any()
+    # equal keys: P = 1 / 4 for the first query and 1 / 5 for the second
+    want = (do[0, 0].double() / 4 + do[0, 1].double() / 5).sum(0)
+    mag = (do[0].double().abs() / 4).sum((0, 1))
+    # (P rounded to bfloat16, lse and exp in float32, the result rounded)
+    assert ((dv[0, 0, 0].double() - want).abs() <= 3 * 2.0 ** -8 * mag).all()
+
+
 def test_results_repeat_bit_for_bit():
     from pstl_diffusion_policy_amd import attention as A
     for shape in ((2, 300, 500, 4, 2, 64), (3, 20, 20, 4, 2, 32), (1, 2, 3000, 8, 2, 128)):

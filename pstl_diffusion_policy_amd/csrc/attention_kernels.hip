@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK > 64 ? 1 : 2) void k_attn
 // Bound by memory: q, k and v pass through the wavefront's LDS tiles and o leaves the same way, so that neighbouring lanes touch
 // neighbouring 16 bytes (fragments read straight from global memory touch 32 rows per instruction: 82 us at 4096 x 12 tokens, 8
 // heads of 32, float32; like this, one unit per wavefront, 59 us; with two units of at most 16 to a wavefront and the values in
-// the keys' place 48 us, 201 MB = 4.2 TB/s).
+// the keys' place 55 us, 201 MB = 3.7 TB/s).
 template <typename T, int DK, bool DROP, bool PAIR>
 __global__ __launch_bounds__(64 * (short_waves<T, DK>(2))) void k_attn_fwd_short(Args a) {
   constexpr int NW = short_waves<T, DK>(2);
@@ -477,7 +477,7 @@ using namespace pstl::attn;
 extern "C" size_t pstl_attention_work_floats(const pstl_attn* c) {
   Args a;
   if (attn_args(c, &a, kCheckShape) != PSTL_OK) return 0;
-  const FwdPlan p = plan_forward(a, device_cus());
+  const FwdPlan p = plan_forward(a, c->dtype == PSTL_F32, device_cus());
   return p.splits > 1 ? (size_t)p.splits * a.B * a.Hk * a.R * (a.D + 2) : 0;
 }
 
@@ -485,7 +485,7 @@ extern "C" int pstl_attention(const pstl_attn* c, void* stream) {
   Args a;
   if (int e = attn_args(c, &a, kCheckForward)) return e;
   if ((int64_t)a.B * a.R == 0) return PSTL_OK;
-  const FwdPlan p = plan_forward(a, device_cus());
+  const FwdPlan p = plan_forward(a, c->dtype == PSTL_F32, device_cus());
   if (p.splits > 1 && !a.part) return PSTL_ERR_ARG;
   if ((int64_t)a.B * a.Hk * p.n_tiles * p.splits >= (1ll << 31)) return PSTL_ERR_SHAPE;
   switch (c->dtype) {

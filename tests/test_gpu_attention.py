@@ -107,6 +107,21 @@ def test_causal_borders(Lq, Lk):
         check_attention(*make(1, Lq, Lk, Hq, Hk, 32, torch.float32, seed=Lq), causal=True)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(33, 12, 300, 8, 4, 32), (33, 50, 70, 4, 4, 64), (17, 130, 290, 8, 4, 80), (33, 40, 270, 4, 4, 128)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_batches_that_fill_the_chip(shape, dtype):
+    """Many sequences: 128-row workgroups, however short; small ones of the same length take 32-row tiles.  With and without masks."""
+    B, Lq, Lk = shape[:3]
+    g = torch.Generator().manual_seed(Lq * 7 + Lk)
+    q, k, v, do = make(B, *shape[1:], dtype, seed=4)
+    check_attention(q, k, v, do)
+    ql = torch.randint(0, Lq + 1, (B,), generator=g, dtype=torch.int32)
+    kl = torch.randint(0, Lk + 1, (B,), generator=g, dtype=torch.int32)
+    mask = torch.rand(B, Lk, generator=g) < 0.6
+    check_attention(q, k, v, do, causal=True, key_mask=mask, q_lens=ql, k_lens=kl, dropout_p=0.25, seed=77)
+
+
 def test_long_sequences():
     check_attention(*make(1, 1500, 1500, 2, 1, 64, torch.bfloat16), causal=True)
     check_attention(*make(2, 1, 20000, 8, 2, 128, torch.float16), train=False, k_lens=torch.tensor([20000, 4097], dtype=torch.int32))

@@ -138,16 +138,16 @@ def test_empty_lengths(Lq, Lk, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
-@pytest.mark.parametrize("Lq, Lk", [(9, 11), (70, 90), (1, 500)])
-def test_hidden_places_may_hold_anything(Lq, Lk, dtype):
+@pytest.mark.parametrize("B, Lq, Lk, D", [(3, 9, 11, 24), (3, 70, 90, 24), (3, 1, 500, 24), (3, 70, 90, 104), (66, 40, 140, 40)])
+def test_hidden_places_may_hold_anything(B, Lq, Lk, D, dtype):
     """NaN and infinities in masked keys, behind the lengths, and in the gradients of rows behind them."""
-    q, k, v, do = make(3, Lq, Lk, 4, 2, 24, dtype)
+    q, k, v, do = make(B, Lq, Lk, 4, 2, D, dtype)
     g = torch.Generator().manual_seed(5)
-    mask = torch.rand(3, Lk, generator=g) < 0.7
-    ql = torch.tensor([Lq, max(Lq // 2, 1), 0], dtype=torch.int32)
-    kl = torch.tensor([Lk, Lk // 3, Lk], dtype=torch.int32)
+    mask = torch.rand(B, Lk, generator=g) < 0.7
+    ql = torch.tensor([Lq, max(Lq // 2, 1), 0] * (B // 3), dtype=torch.int32)
+    kl = torch.tensor([Lk, Lk // 3, Lk] * (B // 3), dtype=torch.int32)
     bad = [math.nan, math.inf, -math.inf]
-    for b in range(3):
+    for b in range(B):
         for i in range(Lq):
             if i >= ql[b]:
                 q[b, i], do[b, i] = bad[i % 3], bad[(i + 1) % 3]
@@ -264,7 +264,7 @@ def test_more_than_2_31_packed_rows_of_keys_behind_the_length():
 
 def test_results_repeat_bit_for_bit():
     from pstl_diffusion_policy_amd import attention as A
-    for shape in ((2, 300, 500, 4, 2, 64), (3, 20, 20, 4, 2, 32), (1, 2, 3000, 8, 2, 128)):
+    for shape in ((2, 300, 500, 4, 2, 64), (2, 300, 500, 4, 2, 128), (3, 20, 20, 4, 2, 32), (1, 2, 3000, 8, 2, 128)):
         q, k, v, do = (t.to(DEV) for t in make(*shape, torch.bfloat16))
         runs = []
         for _ in range(3):
@@ -287,9 +287,20 @@ def test_other_streams_and_two_calls_at_once():
                 outs.append(A.attention(q, k, v))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+    q, k, v, do = (t.to(DEV) for t in make(4, 300, 400, 8, 2, 128, torch.bfloat16))
+    out, lse = A.attention_forward(q, k, v, causal=True)
+    want = A.attention_backward(do, q, k, v, out, lse, causal=True)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(A.attention_backward(do, q, k, v, out, lse, causal=True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
 
 
-@pytest.mark.parametrize("shape", [(2, 20, 20, 4, 2, 32), (2, 150, 200, 4, 2, 64), (1, 1, 5000, 8, 2, 64)])
+@pytest.mark.parametrize("shape", [(2, 20, 20, 4, 2, 32), (2, 150, 200, 4, 2, 64), (2, 150, 200, 4, 2, 128), (1, 1, 5000, 8, 2, 64)])
 def test_captured_step_replays_with_other_seeds(shape):
     """Forward and backward captured in a graph; the seed lives in device memory.  Every replay against the eager result, with eager
     work between the replays; a second graph beside the first."""

@@ -4,6 +4,8 @@ import ctypes
 import math
 import os
 import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -286,3 +288,36 @@ def test_dropout_masks_have_the_rate_and_no_structure():
     whole, _ = ao.dropout_keep(1000, 0.3, seed=5)
     part, _ = ao.dropout_keep(400, 0.3, seed=5, offset=600)
     np.testing.assert_array_equal(whole[600:].numpy(), part.numpy())
+
+
+def test_forward_plans_cover_every_key_and_row(tmp_path):
+    """The choice of the forward kernel, compiled by itself and swept over sizes: every key in one part, every row in one tile, and
+    empty calls divide by nothing."""
+    exe = str(tmp_path / "attn_plan")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                           os.path.join(ROOT, "tests", "hostsim", "attn_plan_main.cpp"), "-o", exe])
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, (run.returncode, run.stdout, run.stderr)
+    assert " 0 failures" in run.stdout
+
+
+def test_empty_calls_need_no_workspace():
+    """No sequence or no query, with more keys than one tile holds.  In a process of its own: a division by zero would end it."""
+    code = """
+import ctypes, sys
+sys.path[:0] = %r
+from test_attention_host import c_attn
+from pstl_diffusion_policy_amd import ffi
+L = ffi.lib()
+for dtype in range(3):
+    for B, Lq in ((0, 3), (2, 0), (0, 0), (0, 200)):
+        for Lk in (0, 5, 32, 33, 100, 128, 256, 300, 100000):
+            none = (0, 0, 0, 0)
+            a = c_attn(dtype=dtype, B=B, Lq=Lq, Lk=Lk, q=none, o=none, work=None, **({"k": none, "v": none} if B == 0 else {}))
+            print(dtype, B, Lq, Lk, flush=True)
+            assert L.pstl_attention_work_floats(ctypes.byref(a)) == 0
+            assert L.pstl_attention(ctypes.byref(a), None) == 0
+print("whole")
+""" % [ROOT, os.path.join(ROOT, "tests")]
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.endswith("whole\n"), (run.returncode, run.stdout[-200:], run.stderr[-2000:])

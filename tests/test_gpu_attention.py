@@ -557,3 +557,15 @@ def test_the_operators_together(dtype):
         err = float((got[i].cpu().double() - want[i]).norm())
         bound = max(float((m[i] - want[i]).norm()) for m in moved) + 4 * u * float(want[i].norm())
         assert err <= bound, (name, err, bound)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Lk", [33, 100, 300])
+@pytest.mark.parametrize("B, Lq", [(0, 3), (2, 0), (0, 0), (0, 200)])
+def test_empty_batches_and_queries_with_many_keys(B, Lq, Lk, dtype):
+    """No sequence or no query where the keys pass one tile: empty results, and zeros as the gradients of keys nobody asked."""
+    for D in (16, 104):
+        q, k, v, do = make(B, Lq, Lk, 4, 2, D, dtype)
+        check_attention(q, k, v, do)
+        check_attention(q, k, v, do, causal=True, key_mask=torch.ones(B, Lk, dtype=torch.bool), dropout_p=0.25, seed=5)

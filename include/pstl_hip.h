@@ -505,8 +505,8 @@ int pstl_qk_norm_rope_backward(const pstl_qk_rope* a, void* stream);
  * Visible: query i < q_lens[b] sees key j < k_lens[b] with key_mask[b mask_stride_b + j] != 0 and, with `causal`,
  * j <= i + k_lens[b] - q_lens[b] (the sequences' ends are aligned).  Lengths (null: full) are clamped to the tensors; masked or
  * out-of-length keys, values and query rows may hold anything, NaN included -- but a value that SOME row of the sequence sees
- * must be finite for the rows that `causal` hides it from.  A row that sees nothing, or i >= q_lens[b], gives o = 0, lse = -inf
- * and no gradient.
+ * must be finite for the rows that `causal` hides it from and that see other keys.  A row that sees nothing, or i >= q_lens[b],
+ * gives o = 0, lse = -inf and dq = 0, whatever the keys and values that other rows see hold.
  * lse (B, Hk, Lq, Hq/Hk) float32, natural logarithm, or null in the forward call; backward reads it.
  * dropout_256: a probability is dropped with dropout_256 / 256 and the kept ones are scaled by 256 / (256 - dropout_256): byte
  * j % 4 of word r % 4 of philox4x32-7(counter = (j / 4, r / 4, b Hk + hk, 0x41545444), key = seed) below dropout_256 drops key j

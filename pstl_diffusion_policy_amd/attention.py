@@ -461,7 +461,7 @@ def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, sc
     A query sees the keys j < k_lens[b] ((B,) int32; Lk) that key_mask ((B, Lk) bool / uint8, true = visible) shows it and, with
     causal, j <= i + k_lens[b] - q_lens[b]: the ends of the sequences are aligned, so a single new query sees its whole cache.
     Queries i >= q_lens[b] and queries that see nothing give zeros, and no gradient.  What is hidden by the mask or lies behind the
-    lengths may hold anything.
+    lengths may hold anything; what only the causal order hides from a query that sees other keys must be finite.
     dropout_p drops probabilities (steps of 1/256; kept ones are scaled by the inverse of the realised keep probability), seed
     draws the mask.  return_lse: also the log of the softmax's sums, (B, Hq, Lq) float32, without a gradient.
     Differentiable in q, k and v; the backward pass forms the probabilities again and is deterministic."""

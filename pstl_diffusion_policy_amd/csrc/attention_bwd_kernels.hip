@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256, (waves_per_simd_q<T, DK>())) void k_attn_bwd_q
     }
   }
   if (r >= a.R) return;
-  if (!live) {
+  if (!live || lse2 == -INFINITY) {      // (a row that sees nothing: selected away, as in the forward kernel)
 #pragma unroll
     for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = f32x16{};
   }
@@ -517,8 +517,9 @@ __global__ __launch_bounds__(64 * (bwd_short_waves<T, DK>()), DK <= 64 ? 2 : 1) 
     qr.load(row_at(a.q), a.D, lane);
     dor.load(row_at(a.dout), a.D, lane);
     const int r = m0 + me.at, qi = row_query(a, r);
-    const bool live = me.ok && r < a.R && qi < n.q;
-    const uint32_t rows_on = (uint32_t)__ballot(live), see = seen_bits<PAIR>(keys_on, live ? row_limit(a, n, qi) : 0, lane);
+    const uint32_t see = seen_bits<PAIR>(keys_on, me.ok && r < a.R ? row_limit(a, n, qi) : 0, lane);
+    const bool live = see != 0;      // (a row that sees nothing is left out, as one behind the length is)
+    const uint32_t rows_on = (uint32_t)__ballot(live);
     const float lse2 = live ? a.lse[(int64_t)me.unit * a.R + r] * kLog2e : 0.0f;
     wave_lds_fence();
     if (m0 == 0) {

@@ -1,7 +1,8 @@
 // attention_kernels.hip -- softmax attention, forward: O = softmax(scale Q K^T) V over padded, ragged, grouped-head batches.
 //
 //   S_rj = scale q_r . k_j,  j < limit(r) and not hidden;   P = exp(S - lse_r),  lse_r = log sum_j exp(S_rj);   O = (m P / keep) V
-// One pass over the keys with the running maximum and sum (32 bits); a row that sees no key gives zeros and lse = -inf.
+// One pass over the keys with the running maximum and sum (32 bits); a row that sees no key gives zeros and lse = -inf: its sum is 0
+// and its result is selected, not multiplied, away (an infinity that other rows of its tile see has come into it as 0 x inf).
 // Scores are formed TRANSPOSED (S^T = K Q^T): a lane holds one row's scores, so that maximum, sum and rescaling need one exchange
 // between the lane halves, and the probabilities are the second operand of O^T = V^T P^T where they stand (attn_core.hpp).
 // Arithmetic: products of 16-bit inputs on v_mfma_f32_32x32x16 with 32-bit sums; the probabilities are rounded to the inputs' type
@@ -150,9 +151,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK > 64 ? 1 : 2) void k_attn
   }
   l = half_sum(l);
   if (r >= a.R) return;
-  const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : l;      // (0 for a row that sees nothing; a NaN sum stays one)
-  if (hi == 0 && a.lse) a.lse[(int64_t)unit * a.R + r] = live && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
-  if (!live) {
+  const bool on = live && l != 0.0f;
+  const float inv = !on ? 0.0f : l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : l;      // (a NaN sum stays one)
+  if (hi == 0 && a.lse) a.lse[(int64_t)unit * a.R + r] = on ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  if (!on) {
 #pragma unroll
     for (int dt = 0; dt < DK / 32; ++dt) acc[dt] = f32x16{};
   }
@@ -230,11 +232,12 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(2))) void k_attn_fwd_short
   f32x16 acc[DK / 32] = {};
   wave_lds_fence();
   contract<T, DK, PAIR>(acc, kt, s, lane);
-  const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : l;      // (0 for a row that sees nothing; a NaN sum stays one)
+  const bool on = live && l != 0.0f;
+  const float inv = l > 0.0f ? (DROP ? a.keep_inv : 1.0f) / l : l;      // (a NaN sum stays one)
   if (hi == 0 && a.lse && me.ok && r < a.R)
-    a.lse[(int64_t)me.unit * a.R + r] = live && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    a.lse[(int64_t)me.unit * a.R + r] = on ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
   wave_lds_fence();
-  RW::from_acc(qt, col, hi, acc, inv, live);
+  RW::from_acc(qt, col, hi, acc, inv, on);
   wave_lds_fence();
   RW::store(qt, row_at(a.o), a.D, lane);
 }
@@ -361,12 +364,12 @@ __global__ __launch_bounds__(256) void k_attn_fwd_few(Args a) {
         st[0] = mr, st[1] = ls;
       }
     } else {
-      const bool lv = row_query(a, rr) < n.q;
+      const bool lv = row_query(a, rr) < n.q && ls != 0.0f;
       const float inv = ls > 0.0f ? (DROP ? a.keep_inv : 1.0f) / ls : ls;
       typedef typename Vec<T>::x4 V4;
       v = lv ? v * inv : f32x4{};
       *reinterpret_cast<V4*>(row_ptr<T>(a, a.o, b, hk, rr) + d) = __builtin_convertvector(v, V4);
-      if (d == 0 && a.lse) a.lse[(int64_t)unit * a.R + rr] = lv && ls != 0.0f ? (mr + __builtin_amdgcn_logf(ls)) * kLn2 : -INFINITY;
+      if (d == 0 && a.lse) a.lse[(int64_t)unit * a.R + rr] = lv ? (mr + __builtin_amdgcn_logf(ls)) * kLn2 : -INFINITY;
     }
   }
 }
@@ -420,9 +423,10 @@ __global__ __launch_bounds__(256) void k_attn_join(Args a, float gain) {
   if (g == 0 && d < a.D) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) v += sums[i][lane];
-    const float inv = l > 0.0f ? gain / l : (l == 0.0f ? 0.0f : l);
+    const float inv = l > 0.0f ? gain / l : l;
     typedef typename Vec<T>::x4 V4;
-    *reinterpret_cast<V4*>(row_ptr<T>(a, a.o, b, hk, r) + d) = __builtin_convertvector(v * inv, V4);
+    v = l != 0.0f ? v * inv : f32x4{};      // (a row that sees nothing)
+    *reinterpret_cast<V4*>(row_ptr<T>(a, a.o, b, hk, r) + d) = __builtin_convertvector(v, V4);
   }
   if (tid == 0 && a.lse) a.lse[row] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }

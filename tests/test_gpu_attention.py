@@ -569,3 +569,37 @@ def test_empty_batches_and_queries_with_many_keys(B, Lq, Lk, dtype):
         q, k, v, do = make(B, Lq, Lk, 4, 2, D, dtype)
         check_attention(q, k, v, do)
         check_attention(q, k, v, do, causal=True, key_mask=torch.ones(B, Lk, dtype=torch.bool), dropout_p=0.25, seed=5)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B, Lq, Lk, Hq, Hk, D", [
+    (3, 9, 11, 2, 2, 24), (3, 20, 30, 4, 2, 40), (3, 70, 20, 4, 2, 64),      # up to 32 keys: in pairs, alone, several row tiles
+    (3, 2, 500, 4, 2, 24), (3, 5, 2000, 4, 2, 104), (3, 8, 600, 4, 4, 64),   # few rows: one part, and divided keys
+    (3, 70, 90, 4, 2, 24), (66, 40, 140, 4, 2, 40), (3, 300, 450, 4, 2, 128)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan], ids=["inf", "nan"])
+def test_rows_that_see_nothing_are_zeros_beside_visible_infinities(B, Lq, Lk, Hq, Hk, D, bad, dtype):
+    """A key or a value that the sequence's other rows see is infinite or NaN: queries behind q_lens, and queries whose causal limit
+    leaves them no key, still give exact zeros, lse = -inf and no gradient."""
+    from pstl_diffusion_policy_amd import attention as A
+    q, k, v, do = make(B, Lq, Lk, Hq, Hk, D, dtype, seed=6)
+    ql = torch.tensor([Lq // 2 + 1, Lq, 1] * (B // 3), dtype=torch.int32)
+    kl = torch.tensor([Lk, max(Lq // 2, 1), Lk] * (B // 3), dtype=torch.int32).clamp(max=Lk)
+    row = torch.arange(Lq)[None]
+    behind = row >= ql[:, None]
+    assert behind.any()
+    for which in (0, 1):
+        bk, bv = k.clone(), v.clone()
+        (bk, bv)[which][:, 0, :, ::3] = bad
+        args = [t.to(DEV) for t in (q, bk, bv)]
+        for causal, p in ((False, 0.0), (True, 0.0), (True, 0.25)):
+            empty = behind | (row < (ql - kl)[:, None]) if causal else behind
+            kw = dict(causal=causal, q_lens=ql.to(DEV), k_lens=kl.to(DEV), dropout_p=p, seed=8)
+            out, lse = A.attention_forward(*args, **kw)
+            dq, dk, dv = A.attention_backward(do.to(DEV), *args, out, lse, **kw)
+            for name, t in (("out", out), ("dq", dq)):
+                t = t.cpu()[empty]
+                assert (t == 0).all(), (name, which, causal, p, int((t != 0).sum()))
+            assert (lse.cpu().permute(0, 2, 1, 3)[empty] == -math.inf).all()
+            assert not out.cpu()[~empty].isfinite().all()                                    # (the others show it)
+            hidden = torch.arange(Lk)[None] >= kl[:, None]
+            assert not dk.cpu()[hidden].any() and not dv.cpu()[hidden].any()

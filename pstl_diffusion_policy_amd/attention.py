@@ -8,10 +8,11 @@ attention_bwd_kernels.hip, token_kernels.hip); tensors are float32, bfloat16 or 
   attention(q, k, v, ...)                                          softmax(scale q k^T) v over padded, ragged, grouped-head batches
   dropout_add(x, p, seed=...)                                      residual + dropout(x); the mask is a function of (seed, element)
 
-The three work under torch.autograd.  `attention_forward` / `attention_backward`, `qk_norm_rope_forward` /
-`qk_norm_rope_backward` and `dropout_backward` are the same calls without autograd, for hosts that sequence launches themselves
-(a training step captured in a HIP graph: engine.GraphCapture).  Every call only enqueues launches on the current stream of the
-tensors' device -- no synchronisation, no host copy -- and can be captured; call it once before capturing.
+The three work under torch.autograd in reverse mode (forward mode raises).  `attention_forward` / `attention_backward`,
+`qk_norm_rope_forward` / `qk_norm_rope_backward` and `dropout_backward` are the same calls without autograd, for hosts that
+sequence launches themselves (a training step captured in a HIP graph: engine.GraphCapture).  Every call only enqueues launches on
+the current stream of the tensors' device -- no synchronisation, no host copy -- and can be captured; call it once before
+capturing.
 
 A seed is an int, or a tensor in device memory that the kernels read when they RUN (int64, one element, or the block of an
 engine.DynBlock): a captured step draws another mask at each replay.  It must keep its value until the backward pass has run.
@@ -22,6 +23,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import ffi
 
@@ -132,6 +134,8 @@ def _needs_grad(*tensors):
         for t in tensors:
             if getattr(t, "requires_grad", False):
                 return True
+    if _forward_ad._current_level >= 0:      # inside a dual_level: a tangent goes through the Function as well, which raises
+        return any(isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
     return False
 
 

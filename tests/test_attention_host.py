@@ -321,3 +321,21 @@ print("whole")
 """ % [ROOT, os.path.join(ROOT, "tests")]
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout.endswith("whole\n"), (run.returncode, run.stdout[-200:], run.stderr[-2000:])
+
+
+def test_a_tangent_asks_for_a_derivative():
+    """Forward mode: a dual tensor has requires_grad False, and the operators, which have no forward-mode formula, must not take it
+    for a constant.  (What they then do needs the GPU.)"""
+    from torch.autograd import forward_ad
+    from pstl_diffusion_policy_amd import attention as A
+    x, plain = torch.ones(4), torch.ones(4)
+    assert not A._needs_grad(x, None, plain)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.full((4,), 2.0))
+        assert not dual.requires_grad
+        assert not A._needs_grad(plain, None)
+        assert A._needs_grad(plain, None, dual) and A._needs_grad(dual)
+        with torch.no_grad():
+            assert A._needs_grad(dual)      # (no_grad stops the backward mode only)
+    assert not A._needs_grad(x, None, plain)
+    assert A._needs_grad(plain.clone().requires_grad_(), None)

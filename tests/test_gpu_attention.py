@@ -603,3 +603,21 @@ def test_rows_that_see_nothing_are_zeros_beside_visible_infinities(B, Lq, Lk, Hq
             assert not out.cpu()[~empty].isfinite().all()                                    # (the others show it)
             hidden = torch.arange(Lk)[None] >= kl[:, None]
             assert not dk.cpu()[hidden].any() and not dv.cpu()[hidden].any()
+
+
+def test_forward_mode_raises_instead_of_dropping_the_tangent():
+    from torch.autograd import forward_ad
+    from pstl_diffusion_policy_amd import attention as A
+    q, k, v, _ = (t.to(DEV) for t in make(2, 4, 6, 2, 2, 16, torch.float32))
+    w, pos, f = torch.ones(16, device=DEV), torch.arange(4, device=DEV), A.rope_frequencies(16).to(DEV)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: A.attention(dual(q), k, v), lambda: A.attention(q, k, dual(v), return_lse=True),
+                 lambda: A.qk_norm_rope(q, dual(q), w, w, pos, f), lambda: A.qk_norm_rope(q, q, dual(w), w, pos, f),
+                 lambda: A.dropout_add(dual(q), 0.5, seed=1), lambda: A.dropout_add(q, 0.5, seed=1, residual=dual(q))]
+        for call in calls:
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                call()
+        with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+            A.attention(dual(q), k, v)
+        assert forward_ad.unpack_dual(A.attention(q, k, v)).tangent is None      # (nothing dual goes in)

@@ -621,3 +621,19 @@ def test_forward_mode_raises_instead_of_dropping_the_tangent():
         with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
             A.attention(dual(q), k, v)
         assert forward_ad.unpack_dual(A.attention(q, k, v)).tangent is None      # (nothing dual goes in)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_weight_gradients_lose_nothing_between_workgroups(dtype):
+    """2048 tokens of one head of ones at position 0 (norm 1, no rotation): every workgroup's part of a weight's gradient is one
+    gradient, exactly.  Their sum, 2^24 and 2047 small whole numbers, is the float64 sum rounded once; sums in 32 bits lose the ones
+    that meet 2^24."""
+    from pstl_diffusion_policy_amd import attention as A
+    g = torch.Generator().manual_seed(2)
+    x = torch.ones(2, 1024, 1, 32).to(DEV, dtype)
+    dy = torch.randint(1, 4, (2, 1024, 1, 32), generator=g).float()
+    dy[0, 0] = 2.0 ** 24
+    w, f = torch.ones(32, device=DEV), A.rope_frequencies(16).to(DEV)
+    _, _, dwq, dwk = A.qk_norm_rope_backward(dy.to(DEV, dtype), -dy.to(DEV, dtype), x, x, w, w, torch.zeros(1024, dtype=torch.int64, device=DEV), f, eps=0.0)
+    want = dy.double().sum((0, 1, 2)).float()
+    assert torch.equal(dwq.cpu(), want) and torch.equal(dwk.cpu(), -want)

@@ -469,7 +469,8 @@ int pstl_refinement(const pstl_cfg* cfg, const float* s0, const float* nei_prep,
  *
  * A pstl_attn_mat is a (B, L, H, D) tensor whose D elements of a row are consecutive: element (b, l, h, d) is
  * p[b stride_b + l stride_l + h stride_h + d] (strides in elements, 64-bit).  p and every row start are 16-byte aligned
- * (PSTL_ERR_ARG otherwise).  Inputs may overlap each other; an output overlaps nothing. */
+ * (PSTL_ERR_ARG otherwise).  Inputs may overlap each other; an output overlaps nothing.  A call of so many rows or elements that a
+ * grid of it would have 2^32 threads is refused whole (PSTL_ERR_SHAPE). */
 enum { PSTL_F32 = 0, PSTL_BF16 = 1, PSTL_F16 = 2 };
 #define PSTL_ATTN_MAX_D 128
 #define PSTL_ROPE_MAX_D 256

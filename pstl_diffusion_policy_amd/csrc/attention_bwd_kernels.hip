@@ -609,6 +609,7 @@ int launch(const Args& a0, hipStream_t st) {
     constexpr int NW = bwd_short_waves<T, DK>();
     const bool pair = in_pairs(a);
     const int64_t jobs = pair ? (units + 1) / 2 : units;
+    if (!grid_fits((jobs + NW - 1) / NW, 64 * NW)) return PSTL_ERR_SHAPE;
     const dim3 grid((unsigned)((jobs + NW - 1) / NW)), block(64 * NW);
     if (pair)
       hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, true, true>), grid, block, 0, st, a);
@@ -618,16 +619,16 @@ int launch(const Args& a0, hipStream_t st) {
       hipLaunchKernelGGL((k_attn_bwd_short<T, DK, DROP, false, false>), grid, block, 0, st, a);
     return launch_status();
   }
+  constexpr bool kDuo = sizeof(T) == 2 && DK > 64;
+  if (!grid_fits(units * ceil_div(a.R, 128), 256) || !grid_fits(units * ceil_div(a.Lk, 64), kDuo ? 512 : 256)) return PSTL_ERR_SHAPE;
   if (a.R > 0) {
     a.n_tiles = ceil_div(a.R, 128);
-    if (units * a.n_tiles >= (1ll << 31)) return PSTL_ERR_SHAPE;
     hipLaunchKernelGGL((k_attn_bwd_q<T, DK, DROP>), dim3((unsigned)(units * a.n_tiles)), dim3(256), 0, st, a);
     if (int e = launch_status()) return e;
   }
   a.n_tiles = ceil_div(a.Lk, 64);
-  if (units * a.n_tiles >= (1ll << 31)) return PSTL_ERR_SHAPE;
   const dim3 grid((unsigned)(units * a.n_tiles));
-  if constexpr (sizeof(T) == 2 && DK > 64) {
+  if constexpr (kDuo) {
     a.cus_per_xcd = 1 << 24;      // one workgroup per compute unit
     constexpr int kBytes = kv_duo_lds<T, DK>();
     if (int e = allow_lds<k_attn_bwd_kv_duo<T, DK, DROP>>(kBytes)) return e;

@@ -437,11 +437,13 @@ int launch(const Args& a0, const FwdPlan& p, hipStream_t st) {
   a.n_tiles = p.n_tiles, a.splits = p.splits, a.tiles_per_split = p.tiles_per_split, a.cus_per_xcd = p.cus_per_xcd;
   const int64_t units = (int64_t)a.B * a.Hk;
   if (p.kind == kManyRows) {
+    if (!grid_fits(units * p.n_tiles, 256)) return PSTL_ERR_SHAPE;
     hipLaunchKernelGGL((k_attn_fwd<T, DK, DROP>), dim3((unsigned)(units * p.n_tiles)), dim3(256), 0, st, a);
   } else if (p.kind == kShort || p.kind == kShortPairs) {
     constexpr int NW = short_waves<T, DK>(2);
     const bool pair = p.kind == kShortPairs;
     const int64_t jobs = (pair ? (units + 1) / 2 : units) * p.n_tiles;
+    if (!grid_fits((jobs + NW - 1) / NW, 64 * NW)) return PSTL_ERR_SHAPE;
     const dim3 grid((unsigned)((jobs + NW - 1) / NW)), block(64 * NW);
     if (pair)
       hipLaunchKernelGGL((k_attn_fwd_short<T, DK, DROP, true>), grid, block, 0, st, a);
@@ -449,6 +451,7 @@ int launch(const Args& a0, const FwdPlan& p, hipStream_t st) {
       hipLaunchKernelGGL((k_attn_fwd_short<T, DK, DROP, false>), grid, block, 0, st, a);
   } else {
     constexpr int kTile2 = 2 * 32 * lds_width(DK) * (int)sizeof(T), kJoin = 32 * DK * 4, kBytes = 4 * (kTile2 > kJoin ? kTile2 : kJoin);
+    if (!grid_fits(units * p.n_tiles * p.splits, 256) || (p.splits > 1 && !grid_fits(units * a.R, 256))) return PSTL_ERR_SHAPE;
     if (int e = allow_lds<k_attn_fwd_few<T, DK, DROP>>(kBytes)) return e;
     hipLaunchKernelGGL((k_attn_fwd_few<T, DK, DROP>), dim3((unsigned)(units * p.n_tiles * p.splits)), dim3(256), kBytes, st, a);
     if (p.splits > 1) {
@@ -491,7 +494,6 @@ extern "C" int pstl_attention(const pstl_attn* c, void* stream) {
   if ((int64_t)a.B * a.R == 0) return PSTL_OK;
   const FwdPlan p = plan_forward(a, c->dtype == PSTL_F32, device_cus());
   if (p.splits > 1 && !a.part) return PSTL_ERR_ARG;
-  if ((int64_t)a.B * a.Hk * p.n_tiles * p.splits >= (1ll << 31)) return PSTL_ERR_SHAPE;
   switch (c->dtype) {
     case PSTL_F32: return launch_dim<float>(a, p, as_stream(stream));
     case PSTL_BF16: return launch_dim<__bf16>(a, p, as_stream(stream));

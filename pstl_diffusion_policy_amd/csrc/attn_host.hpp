@@ -52,6 +52,9 @@ inline int attn_args(const pstl_attn* c, Args* a, Check what) {
   return PSTL_OK;
 }
 
+// does a launch of that many workgroups have fewer than 2^32 threads, the most that a grid can hold?
+inline bool grid_fits(int64_t workgroups, int threads) { return workgroups * threads < (1ll << 32); }
+
 // lets a kernel use `bytes` of dynamic LDS (more than 64 KB must be asked for), once per device
 template <auto Kernel>
 inline int allow_lds(int bytes) {

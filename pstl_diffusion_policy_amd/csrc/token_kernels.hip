@@ -380,7 +380,7 @@ extern "C" int pstl_dropout_add(int dtype, int64_t n, const void* x, const void*
   const uintptr_t el = dtype == PSTL_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) % el) return PSTL_ERR_ARG;
   const int64_t blocks = (n + 2047) / 2048;
-  if (blocks >= (1ll << 31)) return PSTL_ERR_SHAPE;
+  if (!grid_fits(blocks, 256)) return PSTL_ERR_SHAPE;
   DropArgs p = {x, residual, y, n, (uint64_t)offset, (uint64_t)seed, seed_dev, (uint32_t)threshold,
                 threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f};
   const int vec = aligned16(x) && aligned16(y) && aligned16(residual);

@@ -339,3 +339,29 @@ def test_a_tangent_asks_for_a_derivative():
             assert A._needs_grad(dual)      # (no_grad stops the backward mode only)
     assert not A._needs_grad(x, None, plain)
     assert A._needs_grad(plain.clone().requires_grad_(), None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=1, B=1 << 24, Lq=1, Lk=33, Hq=1, Hk=1),             # few rows: a workgroup of 256 per sequence
+    dict(dtype=1, B=1 << 23, Lq=64, Lk=33, Hq=2, Hk=2),            # 128-row workgroups
+    dict(dtype=1, B=1 << 26, Lq=1, Lk=20, Hq=1, Hk=1),             # up to 32 keys: a wavefront per sequence
+    dict(dtype=0, B=1 << 27, Lq=2, Lk=3, Hq=1, Hk=1),              # in pairs
+])
+def test_calls_past_the_largest_grid_are_refused_before_a_launch(kw):
+    """A grid holds fewer than 2^32 threads: such a call is refused by its sizes, whole, and not by a launch that fails half way."""
+    from pstl_diffusion_policy_amd import ffi
+    L = ffi.lib()
+    a = c_attn(D=8, **kw)
+    assert L.pstl_attention(ctypes.byref(a), None) == -2
+    assert L.pstl_attention_backward(ctypes.byref(a), None) == -2
+
+
+def test_dropout_past_the_largest_grid_and_backward_by_keys_alone_are_refused():
+    from pstl_diffusion_policy_amd import ffi
+    L = ffi.lib()
+    one = 1 << 20
+    assert L.pstl_dropout_add(1, 1 << 35, one, None, one, 0, 0, None, 0, None) == -2
+    # few queries, long keys: the queries' grid is small, the keys' is not (16-bit heads over 64 wide: 512 threads a workgroup)
+    for dtype, D, Lk in ((1, 8, (1 << 30) - 64), (0, 8, (1 << 30) - 64), (2, 72, (1 << 29) + 64)):
+        rc = L.pstl_attention_backward(ctypes.byref(c_attn(dtype=dtype, B=1, Lq=1, Lk=Lk, Hq=8, Hk=8, D=D)), None)
+        assert (Lk + 63) // 64 * 8 * (512 if D > 64 else 256) >= 1 << 32 and rc == -2, (dtype, D, rc)

@@ -365,3 +365,42 @@ def test_dropout_past_the_largest_grid_and_backward_by_keys_alone_are_refused():
     for dtype, D, Lk in ((1, 8, (1 << 30) - 64), (0, 8, (1 << 30) - 64), (2, 72, (1 << 29) + 64)):
         rc = L.pstl_attention_backward(ctypes.byref(c_attn(dtype=dtype, B=1, Lq=1, Lk=Lk, Hq=8, Hk=8, D=D)), None)
         assert (Lk + 63) // 64 * 8 * (512 if D > 64 else 256) >= 1 << 32 and rc == -2, (dtype, D, rc)
+
+
+def test_launches_happen_on_the_operands_device(monkeypatch):
+    """The guard around every launch: the operand's device is the current one inside, and the caller's again afterwards, also when the
+    launch raises."""
+    from pstl_diffusion_policy_amd import attention as A
+    state = {"device": 0, "switches": 0}
+
+    class Switch:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state["device"] = state["device"], self.index
+            state["switches"] += 1
+
+        def __exit__(self, *exc):
+            state["device"] = self.before
+
+    class Operand:
+        def __init__(self, index):
+            self.get_device = lambda: index
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["device"])
+    monkeypatch.setattr(torch.cuda, "device", Switch)
+
+    @A._device_guard
+    def launch(q, extra):
+        if extra == "raise":
+            raise RuntimeError("refused")
+        return state["device"], extra
+
+    assert launch(Operand(0), 5) == (0, 5) and state["switches"] == 0      # (already there: nothing is switched)
+    assert launch(Operand(3), 6) == (3, 6) and state == {"device": 0, "switches": 1}
+    with pytest.raises(RuntimeError, match="refused"):
+        launch(Operand(2), "raise")
+    assert state == {"device": 0, "switches": 2}
+    for name in ("_rope_launch", "_attn_forward", "_attn_backward", "_dropout_launch"):
+        assert getattr(A, name).__qualname__.startswith("_device_guard"), name

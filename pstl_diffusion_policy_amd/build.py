@@ -9,12 +9,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libpstl_hip.so")
 ARCH = "gfx950"
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # (source, extra flags).  stl_kernels must not contract mul+add into fma: see csrc/stl_core.hpp.  Its device code is
 # scheduled with the ILP-oriented machine scheduler: the default one serialises chains of packed-fp32 operations through
 # one temporary and pays an s_nop between every two of them (a third of the issue slots of the circle-pair loop);
 # results are bit-identical, the guidance kernel is 3 % faster.
-NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 UNITS = [("stl_kernels.hip", ["-ffp-contract=off", "-Xarch_device", "-mllvm=-misched=gcn-iterative-ilp"]),
          # mlp_kernels: top-down pre-RA list scheduling follows the hand-laid order of the chain kernel's fused block more
          # closely (multi-step launch -1.4 %, single-step -1.9 %, nothing else in the unit changes)

@@ -464,7 +464,7 @@ int pstl_refinement(const pstl_cfg* cfg, const float* s0, const float* nei_prep,
 /* ---- attention over tokens: per-head norm with position rotation, softmax attention, dropout -----------------------
  * Operators for models of tokens (the scene's ego / neighbour / lane tokens, a trajectory's time steps, long sequences), each
  * with its backward pass; they stand beside the token encoders above and share the library's Philox generator with
- * pstl_fill_normal.  Unlike the rest of this header the tensors are of one of three element types, sums are always 32-bit, and
+ * pstl_fill_normal.  Unlike the rest of this header the tensors are of one of three element types, sums have 32 bits or more, and
  * tensors may be strided views.
  *
  * A pstl_attn_mat is a (B, L, H, D) tensor whose D elements of a row are consecutive: element (b, l, h, d) is

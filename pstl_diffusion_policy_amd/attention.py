@@ -2,7 +2,7 @@
 
 Operators for models of tokens (a scene's ego / neighbour / lane tokens, the time steps of a trajectory, long sequences), beside
 the token encoders of engine.Sampler / engine.RectTrainer.  All arithmetic runs in libpstl_hip.so (csrc/attention_kernels.hip,
-attention_bwd_kernels.hip, token_kernels.hip); tensors are float32, bfloat16 or float16, sums are 32-bit whatever the type.
+attention_bwd_kernels.hip, token_kernels.hip); tensors are float32, bfloat16 or float16, sums have 32 bits or more.
 
   qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq)      rotate(w o x / rms(x)) for queries and keys, one launch
   attention(q, k, v, ...)                                          softmax(scale q k^T) v over padded, ragged, grouped-head batches
@@ -466,8 +466,8 @@ def attention(q, k, v, causal=False, key_mask=None, q_lens=None, k_lens=None, sc
     causal, j <= i + k_lens[b] - q_lens[b]: the ends of the sequences are aligned, so a single new query sees its whole cache.
     Queries i >= q_lens[b] and queries that see nothing give zeros, and no gradient.  What is hidden by the mask or lies behind the
     lengths may hold anything; what only the causal order hides from a query that sees other keys must be finite.
-    dropout_p drops probabilities (steps of 1/256; kept ones are scaled by the inverse of the realised keep probability), seed
-    draws the mask.  return_lse: also the log of the softmax's sums, (B, Hq, Lq) float32, without a gradient.
+    dropout_p drops probabilities: it is rounded to the nearest 1/256 (0.1 is 26/256 = 0.1016, 0.01 is 3/256 = 0.0117; what would
+    round to 0 or 1 raises) and kept ones are scaled by the inverse of the realised keep probability; seed draws the mask.  return_lse: also the log of the softmax's sums, (B, Hq, Lq) float32, without a gradient.
     Differentiable in q, k and v; the backward pass forms the probabilities again and is deterministic."""
     if _needs_grad(q, k, v):
         res = _Attention.apply(q, k, v, causal, key_mask, q_lens, k_lens, scale, dropout_p, seed, return_lse)

@@ -40,9 +40,9 @@ __device__ inline float row_dot(const Frag<T> (&x)[DK / 16], const Frag<T> (&y)[
 // ---- dQ: 128 packed rows per workgroup, 32 per wavefront ---------------------------------------------------------------
 // Q, dO and dQ stay in registers, keys and values pass through the LDS as in the forward kernel; 16-bit types run two wavefronts
 // per SIMD, so that one's matrix products stand beside the other's exponentials (one per SIMD with the scores formed a step ahead:
-// 212 us).  4 x 2048 causal, 16/4 heads of 128, bf16: 134 us, 103 GF = 770 TF; the matrix pipe is busy 42 % of the time and the
-// vector pipe 34 %, the rest is LDS latency and the barrier of a tile.  (Copies asked for behind the products instead of right
-// behind the barrier: 135 us.)
+// 212 us).  4 x 2048 causal, 16/4 heads of 128, bf16: 138 us, 103 GF = 750 TF; the matrix pipe is busy 44 % of the time and the
+// vector pipe 35 %, the rest is LDS latency and the barrier of a tile.  (Copies asked for behind the products instead of right
+// behind the barrier: no difference.)
 template <typename T, int DK, bool DROP>
 __global__ __launch_bounds__(256, (waves_per_simd_q<T, DK>())) void k_attn_bwd_q(Args a) {
   constexpr int W = lds_width(DK), BN = block_len<T>(), NS = BN / 32;
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(256, (waves_per_simd_kv<T, DK>())) void k_attn_bwd_
 // marks a dropped probability) through the LDS to w on the same SIMD, which forms dP, dS and dK.  The second kind passes its
 // barrier between dP and dS, the first before S: one is in the matrix pipe while the other forms exponentials.  Copies are asked
 // for behind the first product: 32 KB take 500 cycles to issue, which right behind the barrier nobody had anything to do in.
-// 4 x 2048 causal, 16/4 heads of 128, bf16: 204 us, 137 GF = 670 TF (one wavefront per SIMD with all four: 241 us; both kinds
+// 4 x 2048 causal, 16/4 heads of 128, bf16: 218 us, 137 GF = 630 TF (on the day of these trials 204 us: one wavefront per SIMD with all four: 241 us; both kinds
 // forming S for themselves: 245 us; copies right behind the barrier: 219 us; columns of Q and dO read ahead of the exponentials:
 // no gain).  At D <= 64 everything fits two wavefronts per SIMD in k_attn_bwd_kv, and the handing over only costs (219 -> 226 us).
 template <typename T, int DK>
@@ -473,6 +473,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_bwd_kv_duo(Args a) {
 // as long, turns P and dS through the LDS when there is one row tile (their tiles take the places of V and K): 2048 x 20 tokens,
 // 8 heads of 32, float32, dropout: 112 us (formed twice: 128 us); 294 MB = 2.6 TB/s of 5.0, beside five products of 32 x 32 x 32
 // per unit, 5.4 GF = 35 us at the float32 matrix rate, and the exponentials and draws of 16384 tiles.
+// One wavefront walks ALL rows of its unit: few units with many rows (4096 queries of one sequence on 32 keys, 8 heads: 8
+// wavefronts, 128 tiles one after another) leave most of the chip idle.
 template <typename T, int DK>
 constexpr int bwd_short_waves() {
   return DK <= 32 ? 2 : short_waves<T, DK>(4);

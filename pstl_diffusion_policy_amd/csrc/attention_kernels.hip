@@ -25,9 +25,11 @@ constexpr int block_keys() {
 // values.
 // The maximum that the exponents are taken against moves only when a score exceeds it by more than 2^8: P is then at most 256
 // in 32 bits, the sums stay exact to their rounding, and the accumulators are hardly ever rescaled.
-// Bound by the matrix pipe beside the exponentials of two wavefronts per SIMD.  bf16, causal, 16/4 heads of 128: 8192 tokens 280 us
-// = 985 TF of the 1239 that a large product reaches here; 4 x 2048 tokens 94 us = 730 TF (its 1024 workgroups are two rounds, in
-// which the matrix pipe is busy 41 % and the vector pipe 46 %).  64 rows per wavefront at one wavefront per SIMD: 461 and 150 us;
+// Bound by the matrix pipe beside the exponentials of two wavefronts per SIMD (busy 53 and 52 % at 8192 tokens).  bf16, causal, 16/4
+// heads of 128: 8192 tokens 306 us = 900 TF under the profiler and 278 us a pass without it, 990 TF of the 1239 that a large product
+// reaches here; 4 x 2048 tokens 102 us = 670 TF (its 1024 workgroups are two rounds, in which the matrix pipe is busy 42 % and the
+// vector pipe 46 %).  16-bit heads over 96 wide without dropout spill 7 registers, 32 bytes of scratch a lane: 40 MB written where
+// output and lse are 34.  When these were tried the kernel took 280 and 94 us: 64 rows per wavefront at one wavefront per SIMD: 461 and 150 us;
 // tiles through registers instead of copies: 458 and 107 us; copies asked for behind the products: 330 and 102 us.  float32,
 // 4 x 2048: 727 us, 69 GF = 95 of 153 TF.
 template <typename T, int DK, bool DROP>
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DK > 64 ? 1 : 2) void k_attn
 // Bound by memory: q, k and v pass through the wavefront's LDS tiles and o leaves the same way, so that neighbouring lanes touch
 // neighbouring 16 bytes (fragments read straight from global memory touch 32 rows per instruction: 82 us at 4096 x 12 tokens, 8
 // heads of 32, float32; like this, one unit per wavefront, 59 us; with two units of at most 16 to a wavefront and the values in
-// the keys' place 55 us, 201 MB = 3.7 TB/s).
+// the keys' place 57 us, 201 MB = 3.5 TB/s).
 template <typename T, int DK, bool DROP, bool PAIR>
 __global__ __launch_bounds__(64 * (short_waves<T, DK>(2))) void k_attn_fwd_short(Args a) {
   constexpr int NW = short_waves<T, DK>(2);
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(64 * (short_waves<T, DK>(2))) void k_attn_fwd_short
 // The four wavefronts of a workgroup (and `splits` workgroups) share one set of rows and divide its keys; their results are
 // joined in the LDS (and by k_attn_join).  Bound by reading the keys and values once: tiles of 32 keys are fetched a tile ahead
 // into registers, 16 bytes per lane along the rows, and pass through the wavefront's own LDS tiles.  4 x up to 32768 keys, 16 / 2
-// heads of 128, fp16, 117 MB: 29 us = 4.0 TB/s, and 4 us for the join (two tiles ahead: no gain; one query on 300 keys: 8.5 us,
+// heads of 128, fp16, 117 MB: 30 us = 3.9 TB/s, and 4 us for the join (two tiles ahead: no gain; one query on 300 keys: 8.6 us,
 // latency).
 template <typename T, int DK, bool DROP>
 __global__ __launch_bounds__(256) void k_attn_fwd_few(Args a) {

@@ -13,8 +13,9 @@ namespace {
 // half the rotated width apart, so that both pair orders are rotated inside the thread; `lanes` (a power of two) consecutive
 // lanes make a head.  The angles of a token are shared by all its heads: they are formed once per workgroup, in 64 bits and in
 // revolutions (pos f / 2 pi less its whole part), because a float32 angle of position 10^6 is off by 0.06 rad.
-// 4 x 4096 tokens, 20 heads of 128, bf16: forward 39 us (168 MB = 4.3 TB/s), backward 70 us (252 MB = 3.6 TB/s: its two sums per
-// head and the weights' gradients are vector work beside the loads); 4096 x 20 tokens, 16 heads of 32, float32: 39 and 56 us.
+// 4 x 4096 tokens, 20 heads of 128, bf16: forward 40 us (168 MB = 4.2 TB/s), backward 71 us (252 MB = 3.6 TB/s: its wavefronts wait
+// 75 % of their cycles, because a thread's first loads stand behind the barriers and the angles of its table; the vector pipe is
+// busy half of the time); 2048 x 20 tokens, 16 heads of 32, float32: 41 and 57 us.
 // (Heads summed by shuffles through the LDS and queries' and keys' gradients in one workgroup: 43 and 93 us.)
 struct RopeArgs {
   Mat x[2], y[2], dy[2], dx[2];      // [0] queries, [1] keys
@@ -188,8 +189,9 @@ __global__ __launch_bounds__(256, 4) void k_qk_norm_rope(RopeArgs p) {
 
 // dw[s][d] = sum over the workgroups' parts: one workgroup per (s, 16 elements), 64 strided sums each, joined in a fixed order.  In 64
 // bits: up to 2048 parts of either sign are added one after another, which in 32 bits was most of a weight gradient's error (2.3e-7
-// of its size against 1.1e-7 at 2048 x 20 tokens, 8 heads of 32, float32).  Bound by the latency of its loads: sixteen are in flight per thread (past the end the last part
-// again, not counted: a branch around each load would wait for it before the next, 19 us).  2048 parts of 32 / 128 elements take 4.6 / 5.4 us.
+// of its size against 1.1e-7 at 2048 x 20 tokens, 8 heads of 32, float32).  Bound by the latency of its loads: sixteen are in flight
+// per thread (past the end the last part again, not counted: a branch around each load would wait for it before the next, 19 us).
+// 2048 parts of 32 and 128 elements take 4.6 and 5.3 us.
 __global__ __launch_bounds__(1024) void k_qk_norm_rope_dw(const float* part, int blocks, int D, float* dwq, float* dwk) {
   __shared__ double s[64][16];
   const int lane = threadIdx.x & 15, g = threadIdx.x >> 4, d = (int)blockIdx.x * 16 + lane, which = blockIdx.y;

@@ -6,7 +6,10 @@
 // holds one row: S^T, dP^T, dQ^T; it also leaves delta) and k_attn_bwd_kv or _kv_duo (a lane holds one key: S, dP, dK^T, dV^T;
 // packed rows make the sum over the heads that share a key head part of the same accumulator).  S and dP are formed in both: seven products
 // instead of five, against a second pass over dQ in memory.  Sequences of at most 32 keys have one launch (k_attn_bwd_short).
-// Arithmetic: P and dS are rounded to the inputs' type as operands of dV, dQ and dK; all sums are 32-bit.
+// Arithmetic: P and dS are rounded to the inputs' type as operands of dV, dQ and dK; all sums are 32-bit.  Above 32 keys delta is
+// formed from the rounded O: the sum over d averages its roundings, and the unrounded O would be another tensor to keep for the
+// backward pass.  Error of dQ and dK in bf16, of their size: 0.0025 at 4 x 2048 causal tokens, heads of 128 (their own rounding 0.0017,
+// dS 0.0017, delta 0.0007), 0.0026 at 182 (delta 0.0010: the first rows of a causal call average few values).
 #include "attn_host.hpp"
 
 namespace pstl {
